@@ -110,7 +110,10 @@ def _build_kernels(jobs: int = 8, force: bool = False) -> Path:
     if force and out.exists():
         out.unlink()
     flags = ["-x", "hip", f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden",
-             "-ffast-math", "-fno-finite-math-only", "-munsafe-fp-atomics", f"-I{kdir}"]
+             "-ffast-math", "-fno-finite-math-only", "-munsafe-fp-atomics",
+             # no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32, which the compiler makes of ordinary
+             # float code, have given wrong results on these cards (the host pass does not know the feature and warns)
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", f"-I{kdir}"]
     objs = _compile_objects(srcs, headers, flags, "k", jobs)
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     if force or any(_newer(o, [], out) for o in objs) or _manifest_changed("k", objs):

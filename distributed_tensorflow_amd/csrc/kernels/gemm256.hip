@@ -102,7 +102,7 @@ __device__ __forceinline__ bf16x8_t frag256(const char* half, int row0, int ks, 
 //   gelu(x) = x Phi(x),   gelu'(x) = Phi(x) + x phi(x)
 // Not inlined: spread over the 128 unrolled elements of the epilogue its temporaries push the kernel (already at
 // 240-255 registers) into scratch spills that slow every variant down by 15-30 %.
-// Two elements per call so that the polynomial runs on packed fp32 instructions (v_pk_mul_f32 / v_pk_fma_f32).
+// Two elements per call: their chains interleave (the build has packed fp32 instructions off, see csrc/build.py).
 typedef float f32x2_256 __attribute__((ext_vector_type(2)));
 __device__ __noinline__ f32x4 gelu_pair256(f32x2_256 x) {        // -> {gelu(x0), gelu(x1), gelu'(x0), gelu'(x1)}
   const f32x2_256 xx = x * x * -0.72134752044448170f;
