@@ -1,0 +1,126 @@
+// C entry points of the general attention kernels (attention.h), and the last step of the relative bias's gradient.
+//
+// A call is described by an array of 64-bit words (pointers, element strides, sizes): see the enum. Every entry checks
+// what the kernels assume and returns a negative code without launching anything when it does not hold.
+#include "attention.h"
+
+using namespace dtf;
+
+namespace {
+
+enum Word {
+  kPtr = 0,              // q k v out dout dq dk dv
+  kStride = 8,           // (batch, token, head) strides of the eight, in elements
+  kKeyBias = 32, kLens, kQStart, kQStart0, kTable, kTableBf16, kBuckets, kMaxDist, kBidirectional,
+  kStat, kDelta, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kThr   // then the bucket borders
+};
+
+bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
+  if (n_words < kThr) return false;
+  attn::Strided* t[8] = {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv};
+  for (int i = 0; i < 8; ++i) {
+    t[i]->p = (void*)w[kPtr + i];
+    t[i]->sb = w[kStride + 3 * i];
+    t[i]->ss = w[kStride + 3 * i + 1];
+    t[i]->sh = w[kStride + 3 * i + 2];
+  }
+  a.key_bias = (const float*)w[kKeyBias];
+  a.lens = (const int*)w[kLens];
+  a.q_start = (const int*)w[kQStart];
+  a.q_start0 = (int)w[kQStart0];
+  a.table = (const void*)w[kTable];
+  a.table_bf16 = (int)w[kTableBf16];
+  a.buckets = (int)w[kBuckets];
+  a.max_dist = (int)w[kMaxDist];
+  a.right = w[kBidirectional] ? a.max_dist : 0;
+  a.half = w[kBidirectional] ? a.buckets / 2 : a.buckets;
+  a.exact = a.half / 2;
+  a.stat = (float*)w[kStat];
+  a.delta = (float*)w[kDelta];
+  a.dtab = (float*)w[kDtabParts];
+  const long long lim = 1LL << 30;
+  for (int i = kB; i <= kHd; ++i)
+    if (w[i] <= 0 || w[i] > lim) return false;
+  if (w[kQStart0] > lim || w[kQStart0] < -lim) return false;
+  a.B = (int)w[kB]; a.Sq = (int)w[kSq]; a.Sk = (int)w[kSk]; a.nh = (int)w[kNh]; a.nkv = (int)w[kNkv]; a.hd = (int)w[kHd];
+  a.causal = (int)w[kCausal];
+  a.scale = scale;
+  if (!(scale > 0.f) || scale > 1e30f || a.hd % 8 || a.hd > 128 || a.nh % a.nkv) return false;
+  if (a.table) {
+    a.n_thr = a.half - a.exact - 1;
+    if (a.exact < 1 || a.buckets > 128 || a.max_dist <= a.exact || a.max_dist > 2048 || a.n_thr >= attn::kMaxThr ||
+        n_words < kThr + a.n_thr)
+      return false;
+    for (int i = 0; i < a.n_thr; ++i) a.thr[i] = (int)w[kThr + i];
+  }
+  return true;
+}
+
+// What the kernels read or write through: 16-byte alignment, token strides that hold a row and keep a tile's offsets in
+// 31 bits.
+bool operands_ok(const attn::Args& a, int size, bool backward) {
+  const attn::Strided* t[8] = {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv};
+  const int per16 = 16 / size;
+  for (int i = 0; i < (backward ? 8 : 4); ++i) {
+    if (!t[i]->p || (reinterpret_cast<uintptr_t>(t[i]->p) & 15)) return false;
+    if (t[i]->sb % per16 || t[i]->ss % per16 || t[i]->sh % per16) return false;
+    if (t[i]->sb < 0 || t[i]->sh < 0 || t[i]->ss < a.hd || t[i]->ss > (1 << 22)) return false;
+  }
+  return !backward || (a.stat && a.delta);
+}
+
+bool grid_ok(const attn::Args& a) {
+  const long long q = (long long)a.B * a.nh * ((a.Sq + attn::kRows - 1) / attn::kRows);
+  const long long k = (long long)a.B * a.nkv * ((a.Sk + attn::kRows - 1) / attn::kRows);
+  return q < (1LL << 31) / 256 && k < (1LL << 31) / 256;
+}
+
+// dtable[u, h] = sum over the parts, in a fixed order: one workgroup a head, its threads split the parts.
+__global__ __launch_bounds__(256) void dtab_finish_kernel(const float* __restrict__ parts, void* __restrict__ out,
+                                                         int n_parts, int nh, int buckets, int bf16) {
+  __shared__ float red[256];
+  const int h = blockIdx.x, slices = 256 / buckets, u = threadIdx.x % buckets, s = threadIdx.x / buckets;
+  float v = 0.f;
+  if (s < slices)
+    for (int p = s; p < n_parts; p += slices) v += parts[((long long)p * nh + h) * buckets + u];
+  red[threadIdx.x] = v;
+  __syncthreads();
+  if (s == 0) {
+    for (int i = 1; i < slices; ++i) v += red[i * buckets + u];
+    const long long at = (long long)u * nh + h;
+    if (bf16) ((unsigned short*)out)[at] = f32_to_bf16(v);
+    else ((float*)out)[at] = v;
+  }
+}
+
+}  // namespace
+
+DTF_API int dtf_attention_fwd(const long long* words, int n_words, float scale, hipStream_t stream) {
+  attn::Args a = {};
+  if (!unpack(words, n_words, scale, a)) return -1;
+  const bool bf16 = words[kBf16];
+  if (!operands_ok(a, bf16 ? 2 : 4, false)) return -2;
+  if (!grid_ok(a)) return -3;
+  return bf16 ? attn::fwd_bf16(a, stream) : attn::fwd_f32(a, stream);
+}
+
+// dtab parts: fp32 [B * ceil(Sq / 128)][nh][buckets] scratch; dtab out: [buckets, nh] in the table's type. Both or neither.
+DTF_API int dtf_attention_bwd(const long long* words, int n_words, float scale, hipStream_t stream) {
+  attn::Args a = {};
+  if (!unpack(words, n_words, scale, a)) return -1;
+  const bool bf16 = words[kBf16];
+  if (!operands_ok(a, bf16 ? 2 : 4, true)) return -2;
+  if (!grid_ok(a)) return -3;
+  void* out = (void*)words[kDtabOut];
+  if ((a.dtab != nullptr) != (out != nullptr) || (out && !a.table)) return -4;
+  if (a.dtab) {
+    // four copies of the band of sums where they leave room for a second workgroup on the CU
+    const int band = a.max_dist + a.right + 1 + 2 * attn::kMargin, D = (a.hd + 31) / 32 * 32;
+    a.dtab_copies = attn::lds_tiles(bf16 ? 2 : 4, D) + 4 * (17 * band + 256) <= 80 * 1024 ? 4 : 1;
+  }
+  const int rc = bf16 ? attn::bwd_bf16(a, stream) : attn::bwd_f32(a, stream);
+  if (rc || !a.dtab) return rc;
+  hipLaunchKernelGGL(dtab_finish_kernel, dim3(a.nh), dim3(256), 0, stream, a.dtab, out,
+                     a.B * ((a.Sq + attn::kRows - 1) / attn::kRows), a.nh, a.buckets, a.table_bf16);
+  return (int)hipGetLastError();
+}

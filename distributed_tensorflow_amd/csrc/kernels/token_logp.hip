@@ -1,0 +1,384 @@
+// Log probabilities of given tokens, the entropy, and the top alternatives of each row of logits (gfx950).
+//
+//   lse = log sum_v exp x_v;  logp = x[token] - lse;  H = -sum_v p_v log p_v;  the k largest x_v (ties: lowest index first)
+//   backward: dx_v = -p_v (g_logp + sum_j g_top_j + g_H (log p_v + H)) + g_logp [v = token] + sum_j g_top_j [v = id_j]
+//
+// Bound by the one read of the logits (and one write backward). A workgroup owns a row and walks it in chunks that stay
+// in registers: 4 x 16 bytes a thread.
+//   * With z = x - m and m the running maximum of the THREAD, s = sum e^z and w = sum e^z z need no other thread until
+//     the row ends; H = log s - w / s then has two terms of one sign, so a row that is sure of one token (H near 0) keeps
+//     its digits, which lse - sum p x would not.
+//   * The top k: an element is a candidate when it is no less than a threshold that at least k elements of the row reach.
+//     The first threshold is the k-th largest of 64 maxima over a sixty-fourth of the chunk each, later ones the k-th
+//     best so far: about 1.4 k candidates come out of the first chunk and fewer from each later one, and only they are
+//     ranked. A key of 64 bits (value in an order-preserving code, then the complement of the index) makes every
+//     element's key unique, so the result does not depend on the order in which candidates arrive.
+#include "dtf_common.h"
+
+using namespace dtf;
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kCap = 512;            // candidates held at a time
+constexpr int kMaxTop = 32;
+constexpr int kMaxRows = (1 << 22) - 1;      // 1024 threads a row, below 2^32 in a launch
+constexpr int kMaxCols = 1 << 30;
+constexpr int kU = 4;                // 16-byte vectors a thread holds of a chunk
+constexpr float kFloor = -200.f;     // e^-200 is 0 in fp32: log probabilities are held above it where they meet p
+
+typedef unsigned long long u64;
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int V = 4;
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ float get(const u32x4_t& r, int i) { return __uint_as_float(r[i]); }
+  static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void putv(float* p, const float (&o)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{o[0], o[1], o[2], o[3]}; }
+};
+template <> struct Vec<unsigned short> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ float one(const unsigned short* p) { return bf16_to_f32(*p); }
+  static __device__ __forceinline__ float get(const u32x4_t& r, int i) {
+    return __uint_as_float(i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
+  }
+  static __device__ __forceinline__ void put(unsigned short* p, float v) { *p = f32_to_bf16(v); }
+  static __device__ __forceinline__ void putv(unsigned short* p, const float (&o)[8]) { store8_bf16(p, o); }
+};
+
+// ascending with the value; NaN above everything, -0 equal to +0; equal values descend with the index
+__device__ __forceinline__ u64 key_of(float x, int index) {
+  unsigned b = __float_as_uint(x);
+  if (b == 0x80000000u) b = 0u;
+  unsigned o = (b >> 31) ? ~b : b | 0x80000000u;
+  if (x != x) o = 0xffffffffu;
+  return ((u64)o << 32) | (unsigned)~index;
+}
+__device__ __forceinline__ float value_of(u64 key) {
+  const unsigned o = (unsigned)(key >> 32);
+  return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ u64 shfl_u64(u64 v, int src) {
+  const unsigned lo = __shfl((int)(unsigned)v, src, 64), hi = __shfl((int)(unsigned)(v >> 32), src, 64);
+  return ((u64)hi << 32) | lo;
+}
+__device__ __forceinline__ u64 shfl_xor_u64(u64 v, int m) {
+  const unsigned lo = __shfl_xor((int)(unsigned)v, m, 64), hi = __shfl_xor((int)(unsigned)(v >> 32), m, 64);
+  return ((u64)hi << 32) | lo;
+}
+
+struct Shared {
+  u64 cand[kCap];
+  u64 best[kMaxTop];                 // the k best so far, descending; 0: none
+  u64 group[64];
+  u64 threshold;
+  int count;
+  float red[3][16];
+};
+
+// The k best of best[] (nb of them) and cand[0 .. n), by counting the greater ones: one wave.
+__device__ __forceinline__ void rank_candidates(Shared& sh, int n, int nb, int k, int lane) {
+  constexpr int M = (kCap + kMaxTop + 63) / 64;
+  u64 mine[M];
+  const int total = n + nb;
+#pragma unroll
+  for (int c = 0; c < M; ++c) {
+    const int i = c * 64 + lane;
+    mine[c] = i < n ? sh.cand[i] : (i < total ? sh.best[i - n] : 0ull);
+  }
+  int rank[M] = {};
+  for (int j = 0; j < total; ++j) {
+    const u64 other = j < n ? sh.cand[j] : sh.best[j - n];
+#pragma unroll
+    for (int c = 0; c < M; ++c)
+      if (c * 64 < total) rank[c] += other > mine[c] ? 1 : 0;
+  }
+#pragma unroll
+  for (int c = 0; c < M; ++c)
+    if (c * 64 + lane < total && rank[c] < k) sh.best[rank[c]] = mine[c];
+}
+
+template <typename T, typename L, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict__ x, const L* __restrict__ tokens,
+                                                            float* __restrict__ logp, float* __restrict__ entropy,
+                                                            float* __restrict__ top_logp, long long* __restrict__ top_ids,
+                                                            float* __restrict__ stat, int N, int C, long long ld, int k) {
+  constexpr int V = Vec<T>::V, W = NT / 64;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const long long row = blockIdx.x;
+  const T* xr = x + row * ld;
+  int head = (int)(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / sizeof(T));
+  head = head < C ? head : C;
+  const int nvec = (C - head) / V, tail = C - head - nvec * V;
+  const T* body = xr + head;
+  // the elements before and after the 16-byte vectors: at most V - 1 of each, one a thread
+  const int odd = tid < head ? tid : (tid >= 16 && tid - 16 < tail ? head + nvec * V + tid - 16 : -1);
+  const float xo = odd >= 0 ? Vec<T>::one(xr + odd) : -INFINITY;
+
+  float m = -INFINITY, s = 0.f, w = 0.f;
+  int nb = 0;                                            // entries of sh.best
+  u64 threshold = 0;
+  if (TOP && tid == 0) sh.count = 0;
+  if (TOP) __syncthreads();
+
+  for (int base = 0; base == 0 || base < nvec; base += NT * kU) {
+    u32x4_t r[kU];
+    bool in[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int j = base + u * NT + tid;
+      in[u] = j < nvec;
+      if (in[u]) r[u] = *reinterpret_cast<const u32x4_t*>(body + (long long)j * V);
+    }
+    // running maximum, sum and sum of e^z z of this thread's elements
+    float cm = base == 0 ? xo : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (in[u]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) cm = fmaxf(cm, Vec<T>::get(r[u], i));
+      }
+    const float mn = fmaxf(m, cm), ref = mn == -INFINITY ? 0.f : mn;
+    const float shift = m == -INFINITY ? kFloor : fmaxf(m - ref, kFloor), alpha = __builtin_amdgcn_exp2f(shift * kLog2e);
+    w = alpha * fmaf(s, shift, w);
+    s = alpha * s;
+    m = mn;
+    auto add = [&](float v) {
+      float z = v - ref;
+      z = z < kFloor ? kFloor : z;                       // NaN stays NaN
+      const float e = __builtin_amdgcn_exp2f(z * kLog2e);
+      s += e;
+      w = fmaf(e, z, w);
+    };
+    if (base == 0 && odd >= 0) add(xo);
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (in[u]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) add(Vec<T>::get(r[u], i));
+      }
+    if (!TOP) continue;
+
+    const bool some = in[0] || (base == 0 && odd >= 0);
+    if (base == 0) {
+      // first threshold: k-th largest of 64 maxima. The index in a thread's key is that of its first element where this
+      // is the maximum, otherwise its last one's: no element with the maximum has a lower key. An empty group has key 0
+      u64 key = 0ull;
+      if (some) {
+        const int first = in[0] ? head + tid * V : odd;
+        const float v0 = in[0] ? Vec<T>::get(r[0], 0) : xo;
+        key = key_of(cm, cm == v0 ? first : C + tid);
+      }
+#pragma unroll
+      for (int o = 1; o < W; o <<= 1) {
+        const u64 other = shfl_xor_u64(key, o);
+        key = other > key ? other : key;
+      }
+      if (lane % W == 0) sh.group[wid * (64 / W) + lane / W] = key;
+      __syncthreads();
+      if (wid == 0) {
+        const u64 mine = sh.group[lane];
+        int rank = 0;
+        for (int j = 0; j < 64; ++j) {
+          const u64 other = shfl_u64(mine, j);
+          rank += other > mine || (other == mine && j < lane) ? 1 : 0;
+        }
+        if (rank == k - 1) sh.threshold = mine;
+      }
+      __syncthreads();
+      threshold = sh.threshold;
+    }
+    for (;;) {
+      const float tv = value_of(threshold);
+      // threshold 0: everything passes (value_of(0) is a NaN, which no element is below)
+      const bool scan = some && (!(cm < tv) || s != s);
+      auto offer = [&](float v, int index) {
+        if (v < tv) return;
+        const u64 key = key_of(v, index);
+        if (key < threshold) return;
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kCap) sh.cand[at] = key;
+      };
+      if (scan) {
+        if (base == 0 && odd >= 0) offer(xo, odd);
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (in[u]) {
+            const int first = head + (base + u * NT + tid) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) offer(Vec<T>::get(r[u], i), first + i);
+          }
+      }
+      __syncthreads();
+      const int count = sh.count;
+      __syncthreads();                                   // (the next chunk counts on)
+      if (count == 0) break;
+      if (count <= kCap) {
+        if (wid == 0) rank_candidates(sh, count, nb, k, lane);
+        nb = min(nb + count, k);
+        __syncthreads();
+        if (nb == k) threshold = sh.best[k - 1] + 1;     // later elements have to beat the k-th
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        break;
+      }
+      // too many (whole ranges of equal or ordered values): the k-th best of those held is a higher threshold that k
+      // elements still reach. Take the chunk again with it; at least kCap - k candidates fall away each time
+      u64 kept = lane < nb ? sh.best[lane] : 0ull;       // (every wave saves the list; one writes it back)
+      __syncthreads();
+      if (wid == 0) rank_candidates(sh, kCap, nb, k, lane);
+      __syncthreads();
+      threshold = sh.best[k - 1];
+      __syncthreads();
+      if (wid == 0 && lane < nb) sh.best[lane] = kept;
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+    }
+  }
+
+  // merge the threads' (m, s, w)
+  float gm = wave_max(m);
+  if (lane == 0) sh.red[0][wid] = gm;
+  __syncthreads();
+  gm = sh.red[0][0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) gm = fmaxf(gm, sh.red[0][i]);
+  {
+    const float ref = gm == -INFINITY ? 0.f : gm;
+    const float shift = m == -INFINITY ? kFloor : fmaxf(m - ref, kFloor), alpha = __builtin_amdgcn_exp2f(shift * kLog2e);
+    w = wave_sum(alpha * fmaf(s, shift, w));
+    s = wave_sum(alpha * s);
+  }
+  if (lane == 0) { sh.red[1][wid] = s; sh.red[2][wid] = w; }
+  __syncthreads();
+  s = 0.f;
+  w = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) { s += sh.red[1][i]; w += sh.red[2][i]; }
+  const bool empty = gm == -INFINITY && s == 0.f;        // every logit -inf: no distribution
+  if (wid != 0) return;
+  const float ref = empty ? 0.f : gm, ls = empty ? 0.f : (float)log((double)s);
+  if (lane == 0) {
+    const long long tok = (long long)tokens[row];
+    float lp = 0.f;
+    if (tok >= 0 && tok < C) lp = (Vec<T>::one(xr + tok) - ref) - ls;
+    logp[row] = lp;
+    entropy[row] = empty ? 0.f : ls - w / s;
+    if (stat) {
+      stat[row] = empty ? -INFINITY : gm;
+      stat[(long long)N + row] = ls;
+    }
+  }
+  if (TOP && tid < k) {
+    const u64 key = sh.best[tid];
+    const int index = (int)~(unsigned)key;
+    top_ids[row * k + tid] = index;
+    top_logp[row * k + tid] = (Vec<T>::one(xr + index) - ref) - ls;
+  }
+}
+
+template <typename T, typename L, int NT>
+__global__ __launch_bounds__(NT) void token_logp_bwd_kernel(const T* __restrict__ x, const L* __restrict__ tokens,
+                                                            const float* __restrict__ stat, const float* __restrict__ entropy,
+                                                            const long long* __restrict__ top_ids,
+                                                            const float* __restrict__ g_logp, const float* __restrict__ g_ent,
+                                                            const float* __restrict__ g_top, T* __restrict__ dx, int N, int C,
+                                                            long long ld, int k) {
+  constexpr int V = Vec<T>::V;
+  __shared__ int ids[kMaxTop];
+  __shared__ float gts[kMaxTop];
+  const int tid = threadIdx.x;
+  const long long row = blockIdx.x;
+  const T* xr = x + row * ld;
+  T* dr = dx + row * ld;
+  const float m = stat[row], ls = stat[(long long)N + row], H = entropy[row];
+  const long long tok64 = (long long)tokens[row];
+  const int tok = tok64 >= 0 && tok64 < C ? (int)tok64 : -1;
+  const float ga = g_logp && tok >= 0 ? g_logp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
+  if (tid < k) {
+    ids[tid] = (int)top_ids[row * k + tid];
+    gts[tid] = g_top[row * k + tid];
+  }
+  __syncthreads();
+  float all = ga;
+  for (int j = 0; j < k; ++j) all += gts[j];
+  // d = p (A + B log p), A = -(g_logp + sum g_top + g_H H), B = -g_H; a row without a distribution has no gradient
+  const bool empty = m == -INFINITY;
+  const float A = -fmaf(gh, H, all), B = -gh;
+  auto grad = [&](float v) {
+    float lp = (v - m) - ls;
+    lp = lp < kFloor ? kFloor : lp;
+    return empty ? 0.f : __builtin_amdgcn_exp2f(lp * kLog2e) * fmaf(B, lp, A);
+  };
+  int head = (int)(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / sizeof(T));
+  head = head < C ? head : C;
+  const int nvec = (C - head) / V;
+  if (tid < head) Vec<T>::put(dr + tid, grad(Vec<T>::one(xr + tid)));
+  for (int j = tid; j < nvec; j += NT) {
+    const u32x4_t r = *reinterpret_cast<const u32x4_t*>(xr + head + (long long)j * V);
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = grad(Vec<T>::get(r, i));
+    Vec<T>::putv(dr + head + (long long)j * V, o);
+  }
+  for (int i = head + nvec * V + tid; i < C; i += NT) Vec<T>::put(dr + i, grad(Vec<T>::one(xr + i)));
+  for (long long i = C + tid; i < ld; i += NT) Vec<T>::put(dr + i, 0.f);      // padding between the rows
+  if (empty) return;
+  drain_stores();
+  __syncthreads();
+  // the elements that are the token or an alternative are written again, with their own terms
+  if (tid < k) {
+    const int v = ids[tid];
+    Vec<T>::put(dr + v, grad(Vec<T>::one(xr + v)) + gts[tid] + (v == tok ? ga : 0.f));
+  } else if (tid == k && tok >= 0) {
+    bool listed = false;
+    for (int j = 0; j < k; ++j) listed |= ids[j] == tok;
+    if (!listed) Vec<T>::put(dr + tok, grad(Vec<T>::one(xr + tok)) + ga);
+  }
+}
+
+}  // namespace
+
+// x [N, C] (row stride ld >= C; 0 fp32, 1 bf16), tokens [N] (0 int32, 1 int64; outside [0, C): logp 0), 0 <= k <= 32, k <= C.
+// top_logp / top_ids [N, k] (unused when k is 0), stat (optional): fp32 [2, N] for the backward pass.
+DTF_API int dtf_token_logp_fwd(const void* x, const void* tokens, float* logp, float* entropy, float* top_logp,
+                               long long* top_ids, float* stat, int N, int C, long long ld, int k, int x_dtype,
+                               int label_dtype, hipStream_t stream) {
+  if (N <= 0) return 0;
+  if (C <= 0 || ld < C || k < 0 || k > kMaxTop || k > C || N > kMaxRows || C > kMaxCols) return -1;
+#define FWD(T, L, NT, TOP)                                                                                            \
+  hipLaunchKernelGGL((token_logp_fwd_kernel<T, L, NT, TOP>), dim3(N), dim3(NT), 0, stream, (const T*)x, (const L*)tokens, \
+                     logp, entropy, top_logp, top_ids, stat, N, C, ld, k)
+#define FWD_L(T, L) \
+  if (C > 8192) { if (k) FWD(T, L, 1024, true); else FWD(T, L, 1024, false); } else { if (k) FWD(T, L, 256, true); else FWD(T, L, 256, false); }
+  if (x_dtype == 0 && label_dtype == 0) { FWD_L(float, int) }
+  else if (x_dtype == 0) { FWD_L(float, long long) }
+  else if (label_dtype == 0) { FWD_L(unsigned short, int) }
+  else { FWD_L(unsigned short, long long) }
+#undef FWD_L
+#undef FWD
+  return (int)hipGetLastError();
+}
+
+// dx has x's row stride and its alignment modulo 16 bytes. A gradient may be null (0); g_top is needed when k > 0.
+DTF_API int dtf_token_logp_bwd(const void* x, const void* tokens, const float* stat, const float* entropy,
+                               const long long* top_ids, const float* g_logp, const float* g_ent, const float* g_top, void* dx,
+                               int N, int C, long long ld, int k, int x_dtype, int label_dtype, hipStream_t stream) {
+  if (N <= 0) return 0;
+  if (C <= 0 || ld < C || k < 0 || k > kMaxTop || k > C || N > kMaxRows || C > kMaxCols || (k && (!g_top || !top_ids)))
+    return -1;
+  if ((reinterpret_cast<uintptr_t>(x) & 15) != (reinterpret_cast<uintptr_t>(dx) & 15)) return -2;
+#define BWD(T, L, NT)                                                                                                  \
+  hipLaunchKernelGGL((token_logp_bwd_kernel<T, L, NT>), dim3(N), dim3(NT), 0, stream, (const T*)x, (const L*)tokens, stat, \
+                     entropy, top_ids, g_logp, g_ent, g_top, (T*)dx, N, C, ld, k)
+#define BWD_L(T, L) if (C > 8192) BWD(T, L, 1024); else BWD(T, L, 256);
+  if (x_dtype == 0 && label_dtype == 0) { BWD_L(float, int) }
+  else if (x_dtype == 0) { BWD_L(float, long long) }
+  else if (label_dtype == 0) { BWD_L(unsigned short, int) }
+  else { BWD_L(unsigned short, long long) }
+#undef BWD_L
+#undef BWD
+  return (int)hipGetLastError();
+}

@@ -10,6 +10,7 @@ library is missing, :func:`kernels` raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -100,6 +101,20 @@ def stream_ptr(device=None) -> ctypes.c_void_p:
             idx = device.index if device.index is not None else torch.cuda.current_device()
         return ctypes.c_void_p(_raw_stream(idx))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+@contextlib.contextmanager
+def _device(t: torch.Tensor):
+    with torch.cuda.device(t.device):
+        yield
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Makes ``t``'s GPU the current one for a launch on it (the kernels use the current device's context)."""
+    return _here if t.device.index == torch.cuda.current_device() else _device(t)
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -10,10 +10,15 @@ gradient the reference's ``tape.gradient`` of that vector computes
 loss to softmax *probabilities* clipped to ``[eps, 1 - eps]`` and renormalised
 (what Keras does for ``from_logits=False``); it runs in plain torch since it is
 a parity option for 10-class outputs, not a hot path.
+
+``token_log_probs(logits, tokens, top=k)`` scores given tokens: their log
+probabilities, the entropy of each row and its ``k`` best alternatives, in one
+pass over the logits, with gradients (front end of ``csrc/kernels/token_logp.hip``).
 """
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -129,3 +134,96 @@ def softmax_ce_eval(logits: torch.Tensor, labels: torch.Tensor):
         labels = labels.reshape(-1)
     _, _, loss, _, correct = _fwd(logits, labels, True)
     return loss, correct
+
+
+class TokenLogProbs(NamedTuple):
+    logp: torch.Tensor       # log probability of the token
+    entropy: torch.Tensor    # of the row's distribution, in nats
+    top_logp: torch.Tensor   # [..., top], descending
+    top_ids: torch.Tensor    # [..., top] int64
+
+
+MAX_TOP = 32
+
+
+class _TokenLogp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        x = logits if _row_padded(logits) else logits.contiguous()
+        N, C = x.shape
+        ld = x.stride(0) if N > 1 else C
+        y, dev = tokens.contiguous(), x.device
+        logp, entropy = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
+        stat = torch.empty(2, N, dtype=torch.float32, device=dev)        # row maximum, log of the row's sum above it
+        top_logp = torch.empty(N, top, dtype=torch.float32, device=dev)
+        top_ids = torch.empty(N, top, dtype=torch.int64, device=dev)
+        with _lib.on_device(x):
+            rc = _lib.kernels().dtf_token_logp_fwd(_lib.ptr(x), _lib.ptr(y), _lib.ptr(logp), _lib.ptr(entropy),
+                                                   _lib.ptr(top_logp), _lib.ptr(top_ids), _lib.ptr(stat), N, C,
+                                                   ctypes.c_longlong(ld), top, _lib.dtype_code(x.dtype), _label_code(y),
+                                                   _lib.stream_ptr(dev))
+        _lib.check(rc, "token_logp_fwd")
+        ctx.save_for_backward(x, y, stat, entropy, top_ids)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_ent, g_top, _):
+        x, y, stat, entropy, top_ids = ctx.saved_tensors
+        if g_logp is None and g_ent is None and g_top is None:
+            return None, None, None
+        g_logp, g_ent, g_top = (None if g is None else g.float().contiguous() for g in (g_logp, g_ent, g_top))
+        N, C = x.shape
+        ld = x.stride(0) if N > 1 else C
+        # the rows of dx as those of x, in stride and in alignment
+        shift = x.data_ptr() % 16 // x.element_size()
+        dx = torch.empty(N * ld + shift, dtype=x.dtype, device=x.device)[shift:].view(N, ld)[:, :C]
+        k = 0 if g_top is None else top_ids.shape[1]
+        with _lib.on_device(x):
+            rc = _lib.kernels().dtf_token_logp_bwd(_lib.ptr(x), _lib.ptr(y), _lib.ptr(stat), _lib.ptr(entropy), _lib.ptr(top_ids),
+                                                   _lib.ptr(g_logp), _lib.ptr(g_ent), _lib.ptr(g_top), _lib.ptr(dx), N, C,
+                                                   ctypes.c_longlong(ld), k, _lib.dtype_code(x.dtype), _label_code(y),
+                                                   _lib.stream_ptr(x.device))
+        _lib.check(rc, "token_logp_bwd")
+        return dx, None, None
+
+
+def _token_logp_composed(logits, tokens, top):
+    x = logits.float()
+    ok = (tokens >= 0) & (tokens < x.shape[1])
+    best = x.detach().amax(1, keepdim=True)
+    none = best == -torch.inf                       # a row without a distribution: entropy 0, no gradient
+    z = torch.where(none, x.detach(), x) - best.masked_fill(none, 0.0)
+    total = z.exp().sum(1, keepdim=True)
+    lp = z - total.masked_fill(none, 1.0).log()
+    logp = torch.where(ok, lp.gather(1, tokens.clamp(0, x.shape[1] - 1).long()[:, None])[:, 0], 0.0)
+    seen = lp != -torch.inf
+    entropy = -(lp.exp() * torch.where(seen, lp, 0.0)).sum(1)
+    top_ids = torch.sort(x.detach(), dim=1, descending=True, stable=True).indices[:, :top]
+    return logp, entropy, lp.gather(1, top_ids), top_ids
+
+
+def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogProbs:
+    """Scores ``tokens[...]`` (int32 or int64) under ``logits[..., V]`` (float32 or bfloat16): ``logp``, ``entropy``,
+    ``top_logp`` in float32 and ``top_ids``, all shaped like ``tokens`` (the last two with ``top`` more, at most 32).
+
+    A token outside ``[0, V)`` (an ignored position) has ``logp`` 0 and no gradient through it. Alternatives of equal
+    logits come lowest index first. Logits of -inf are words that cannot be; in a row of nothing else the log
+    probabilities are -inf, the entropy 0 and the gradients 0. The three floating results have gradients."""
+    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
+        raise ValueError(f"logits [..., V] and tokens [...] do not fit: {tuple(logits.shape)}, {tuple(tokens.shape)}")
+    if logits.device != tokens.device:
+        raise ValueError(f"logits are on {logits.device}, tokens on {tokens.device}")
+    _lib.dtype_code(logits.dtype)
+    _label_code(tokens)
+    V, shape = logits.shape[-1], tokens.shape
+    if not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"top {top}: need 0 to {MAX_TOP}, and no more than the {V} logits of a row")
+    if V < 1 or V > 1 << 30 or tokens.numel() >= 1 << 22:
+        raise ValueError(f"{tokens.numel()} rows of {V} logits: need at least 1 logit a row and fewer than {1 << 22} rows")
+    x, y = logits.reshape(-1, V), tokens.reshape(-1)
+    run = _TokenLogp.apply if x.is_cuda and y.numel() else _token_logp_composed
+    r = run(x, y, int(top))
+    return TokenLogProbs(r[0].view(shape), r[1].view(shape), r[2].view(*shape, top), r[3].view(*shape, top))
