@@ -81,8 +81,10 @@ __global__ __launch_bounds__(256) void dtab_finish_kernel(const float* __restric
   __shared__ float red[256];
   const int h = blockIdx.x, slices = 256 / buckets, u = threadIdx.x % buckets, s = threadIdx.x / buckets;
   float v = 0.f;
-  if (s < slices)
+  if (s < slices) {
+#pragma unroll 8
     for (int p = s; p < n_parts; p += slices) v += parts[((long long)p * nh + h) * buckets + u];
+  }
   red[threadIdx.x] = v;
   __syncthreads();
   if (s == 0) {
@@ -113,11 +115,6 @@ DTF_API int dtf_attention_bwd(const long long* words, int n_words, float scale, 
   if (!grid_ok(a)) return -3;
   void* out = (void*)words[kDtabOut];
   if ((a.dtab != nullptr) != (out != nullptr) || (out && !a.table)) return -4;
-  if (a.dtab) {
-    // four copies of the band of sums where they leave room for a second workgroup on the CU
-    const int band = a.max_dist + a.right + 1 + 2 * attn::kMargin, D = (a.hd + 31) / 32 * 32;
-    a.dtab_copies = attn::lds_tiles(bf16 ? 2 : 4, D) + 4 * (17 * band + 256) <= 80 * 1024 ? 4 : 1;
-  }
   const int rc = bf16 ? attn::bwd_bf16(a, stream) : attn::bwd_f32(a, stream);
   if (rc || !a.dtab) return rc;
   hipLaunchKernelGGL(dtab_finish_kernel, dim3(a.nh), dim3(256), 0, stream, a.dtab, out,

@@ -12,7 +12,7 @@ using namespace dtf;
 
 namespace {
 
-constexpr int kMaxThr = 64, kRowsPerBlock = 32;
+constexpr int kMaxThr = 64;
 
 struct BiasArgs {
   int Sq, Sk, heads, start, buckets, half, exact, max_dist, right, n_thr, thr[kMaxThr];
@@ -26,6 +26,16 @@ __device__ __forceinline__ int bucket_of(const BiasArgs& a, int dist) {
     for (int t = 0; t < a.n_thr; ++t) b += far >= a.thr[t] ? 1 : 0;
   }
   return b + (a.right && dist > 0 ? a.half : 0);
+}
+
+// the distances of bucket u, inclusive (none: lo > hi)
+__device__ __forceinline__ void bucket_range(const BiasArgs& a, int u, int& lo, int& hi) {
+  const bool pos = a.right && u >= a.half;
+  const int t = pos ? u - a.half : u, far = 0x3fffffff;
+  const int from = t <= a.exact ? t : a.thr[t - a.exact - 1];
+  const int to = t == a.half - 1 ? far : (t < a.exact ? t : a.thr[t - a.exact] - 1);
+  lo = pos ? (from < 1 ? 1 : from) : -to;
+  hi = pos ? to : (!a.right && t == 0 ? far : -from);
 }
 
 template <typename T>
@@ -42,47 +52,94 @@ __global__ __launch_bounds__(256) void bias_fwd_kernel(BiasArgs a, const T* __re
   }
 }
 
-__device__ __forceinline__ float as_float(unsigned short v) { return bf16_to_f32(v); }
-__device__ __forceinline__ float as_float(float v) { return v; }
-
-// One workgroup: kRowsPerBlock rows of one head. A thread owns distances, not columns, and adds their elements row after
-// row: every sum has a fixed order.
-template <typename T>
-__global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, const T* __restrict__ g, float* __restrict__ parts) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* band = reinterpret_cast<float*>(smem);          // sums of the distances -max_dist .. right
-  const int tid = threadIdx.x, h = blockIdx.y;
-  const int i0 = blockIdx.x * kRowsPerBlock, i1 = min(i0 + kRowsPerBlock, a.Sq);
-  float far_l = 0.f, far_r = 0.f;
-  for (int d = tid; d <= a.max_dist + a.right; d += 256) {
-    float v = 0.f;
-    for (int i = i0; i < i1; ++i) {
-      const int j = a.start + i + d - a.max_dist;
-      if (j >= 0 && j < a.Sk && d > 0 && d < a.max_dist + a.right) v += as_float(g[((long long)h * a.Sq + i) * a.Sk + j]);
-    }
-    band[d] = v;
+// 8 elements of a row from column j on; zero from column n on. The rows have any alignment: the load is left to the
+// compiler, which reads 16 bytes at once at an address of any alignment.
+__device__ __forceinline__ void load8(const unsigned short* row, int j, int n, float (&o)[8]) {
+  if (j + 8 <= n) {
+    u16x8 v;
+    __builtin_memcpy(&v, row + j, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = bf16_to_f32(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = j + i < n ? bf16_to_f32(row[j + i]) : 0.f;
   }
-  for (int i = i0; i < i1; ++i) {
-    const T* row = g + ((long long)h * a.Sq + i) * a.Sk;
-    const int pos = a.start + i;
-    const int left = min(max(pos - a.max_dist + 1, 0), a.Sk), right = min(max(pos + a.right, left), a.Sk);
-    for (int j = tid; j < left; j += 256) far_l += as_float(row[j]);
-    for (int j = right + tid; j < a.Sk; j += 256) far_r += as_float(row[j]);
+}
+__device__ __forceinline__ void load8(const float* row, int j, int n, float (&o)[8]) {
+  if (j + 8 <= n) {
+    __builtin_memcpy(o, row + j, 32);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = j + i < n ? row[j + i] : 0.f;
+  }
+}
+
+// A wave takes tiles of 8 rows x 512 columns, a lane 8 x 8 of them: 64 elements on 15 diagonals, which it adds up in
+// registers. Where the 15 distances are all on one far side (most of a long row) they go into one register; on the band
+// they go to the wave's own LDS sums, 15 additions with the lanes 8 distances apart (the sums are stored by distance
+// modulo 8 first, so that they fall on neighbouring banks). No sum depends on another wave: the order is fixed.
+template <typename T>
+__global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, const T* __restrict__ g, float* __restrict__ parts,
+                                                       int tiles_per_wave, int col_tiles, long long n_tiles) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, h = blockIdx.y;
+  const int n = a.max_dist + a.right + 1, eighth = (n + 14) / 8 + 1, size = eighth * 8;   // distances -max_dist - 7 ..
+  float* sums = reinterpret_cast<float*>(smem) + wid * size;
+  for (int i = lane; i < size; i += 64) sums[i] = 0.f;
+  float far_l = 0.f, far_r = 0.f;
+  const long long first = ((long long)blockIdx.x * 4 + wid) * tiles_per_wave;
+  for (long long t = first; t < first + tiles_per_wave && t < n_tiles; ++t) {
+    const int i0 = (int)(t / col_tiles) * 8, j0 = (int)(t % col_tiles) * 512 + lane * 8;
+    float acc[15];
+#pragma unroll
+    for (int d = 0; d < 15; ++d) acc[d] = 0.f;
+    const T* row = g + ((long long)h * a.Sq + i0) * a.Sk;
+    if (j0 < a.Sk) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (i0 + r < a.Sq) {
+          float v[8];
+          load8(row + (long long)r * a.Sk, j0, a.Sk, v);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) acc[c - r + 7] += v[c];
+        }
+    }
+    const int low = j0 - (a.start + i0) - 7;                               // distance of acc[0]
+    if (low + 14 <= -a.max_dist || low >= a.right) {
+      float v = 0.f;
+#pragma unroll
+      for (int d = 0; d < 15; ++d) v += acc[d];
+      if (low < 0) far_l += v; else far_r += v;
+    } else {
+#pragma unroll
+      for (int d = 0; d < 15; ++d) {
+        // (distances beyond the borders belong to the outermost entries' buckets like these)
+        const int i = min(max(low + d, -a.max_dist), a.right) + a.max_dist;
+        if (low + d <= -a.max_dist) far_l += acc[d];
+        else if (low + d >= a.right) far_r += acc[d];
+        else sums[(i & 7) * eighth + (i >> 3)] += acc[d];
+      }
+    }
   }
   __shared__ float scratch[16];
   far_l = block_sum(far_l, scratch);
   far_r = block_sum(far_r, scratch);
   __syncthreads();
-  if (tid == 0) {
-    band[0] += far_l;
-    band[a.max_dist + a.right] += far_r;
-  }
+  float* all = reinterpret_cast<float*>(smem);
+  for (int i = tid; i < size; i += 256) all[i] = (all[i] + all[size + i]) + (all[2 * size + i] + all[3 * size + i]);
   __syncthreads();
-  for (int u = tid; u < a.buckets; u += 256) {
+  if (tid < a.buckets) {
+    // the distances of this bucket that lie strictly between the borders, then the far sums
     float v = 0.f;
-    for (int d = 0; d <= a.max_dist + a.right; ++d)
-      if (bucket_of(a, d - a.max_dist) == u) v += band[d];
-    parts[((long long)blockIdx.x * a.heads + h) * a.buckets + u] = v;
+    int lo, hi;
+    bucket_range(a, tid, lo, hi);
+    for (int d = max(lo, 1 - a.max_dist); d <= min(hi, a.right - 1); ++d) {
+      const int i = d + a.max_dist;
+      v += all[(i & 7) * eighth + (i >> 3)];
+    }
+    if (lo <= -a.max_dist && hi >= -a.max_dist) v += far_l;
+    if (hi >= a.right && lo <= a.right) v += far_r;
+    parts[((long long)blockIdx.x * a.heads + h) * a.buckets + tid] = v;
   }
 }
 
@@ -92,8 +149,10 @@ __global__ __launch_bounds__(256) void bias_finish_kernel(const float* __restric
   __shared__ float red[256];
   const int h = blockIdx.x, slices = 256 / buckets, u = threadIdx.x % buckets, s = threadIdx.x / buckets;
   float v = 0.f;
-  if (s < slices)
+  if (s < slices) {
+#pragma unroll 8
     for (int p = s; p < n_parts; p += slices) v += parts[((long long)p * heads + h) * buckets + u];
+  }
   red[threadIdx.x] = v;
   __syncthreads();
   if (s == 0) {
@@ -119,6 +178,11 @@ bool unpack(const long long* w, int n, BiasArgs& a) {
   return true;
 }
 
+int tiles_per_wave(long long tiles, int heads) {
+  const long long per = tiles * heads / (256 * 32);
+  return (int)(per < 1 ? 1 : per);
+}
+
 }  // namespace
 
 DTF_API int dtf_relative_bias_fwd(const long long* words, int n_words, const void* table, void* out, int dtype,
@@ -132,18 +196,30 @@ DTF_API int dtf_relative_bias_fwd(const long long* words, int n_words, const voi
   return (int)hipGetLastError();
 }
 
-// Partial sums that the backward pass writes, in units of buckets * heads floats.
-DTF_API int dtf_relative_bias_parts(int Sq, int Sk) { return (Sq + kRowsPerBlock - 1) / kRowsPerBlock; }
+// Partial sums that the backward pass writes, in units of buckets * heads floats: one for each workgroup of a head. About
+// eight waves a SIMD over all heads, each with as many tiles as that takes.
+DTF_API int dtf_relative_bias_parts(int Sq, int Sk, int heads) {
+  const long long tiles = (long long)((Sq + 7) / 8) * ((Sk + 511) / 512);
+  const int per_wave = tiles_per_wave(tiles, heads);
+  return (int)((tiles + 4LL * per_wave - 1) / (4LL * per_wave));
+}
 
 DTF_API int dtf_relative_bias_bwd(const long long* words, int n_words, const void* g, float* parts, void* dtable, int dtype,
                                   hipStream_t stream) {
   BiasArgs a = {};
   if (!unpack(words, n_words, a)) return -1;
-  const int n_parts = dtf_relative_bias_parts(a.Sq, a.Sk);
+  const int n_parts = dtf_relative_bias_parts(a.Sq, a.Sk, a.heads), col_tiles = (a.Sk + 511) / 512;
+  const long long n_tiles = (long long)((a.Sq + 7) / 8) * col_tiles;
+  const int per = tiles_per_wave(n_tiles, a.heads);
   const dim3 grid((unsigned)n_parts, (unsigned)a.heads);
-  const size_t lds = (size_t)(a.max_dist + a.right + 1) * 4;
-  if (dtype) hipLaunchKernelGGL(bias_bwd_kernel<unsigned short>, grid, dim3(256), lds, stream, a, (const unsigned short*)g, parts);
-  else hipLaunchKernelGGL(bias_bwd_kernel<float>, grid, dim3(256), lds, stream, a, (const float*)g, parts);
+  const size_t lds = (size_t)((a.max_dist + a.right + 1 + 14) / 8 + 1) * 8 * 4 * 4;
+  const void* kernel = dtype ? (const void*)bias_bwd_kernel<unsigned short> : (const void*)bias_bwd_kernel<float>;
+  if (lds > 64 * 1024) {
+    const int rc = (int)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (rc) return rc;
+  }
+  if (dtype) hipLaunchKernelGGL(bias_bwd_kernel<unsigned short>, grid, dim3(256), lds, stream, a, (const unsigned short*)g, parts, per, col_tiles, n_tiles);
+  else hipLaunchKernelGGL(bias_bwd_kernel<float>, grid, dim3(256), lds, stream, a, (const float*)g, parts, per, col_tiles, n_tiles);
   if (dtype) hipLaunchKernelGGL(bias_finish_kernel<unsigned short>, dim3(a.heads), dim3(256), 0, stream, parts, (unsigned short*)dtable, n_parts, a.heads, a.buckets);
   else hipLaunchKernelGGL(bias_finish_kernel<float>, dim3(a.heads), dim3(256), 0, stream, parts, (float*)dtable, n_parts, a.heads, a.buckets);
   return (int)hipGetLastError();

@@ -21,6 +21,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCap = 512;            // candidates held at a time
+constexpr int kKeep = 40;            // with up to 24 alternatives they are ranked in one wave
 constexpr int kMaxTop = 32;
 constexpr int kMaxRows = (1 << 22) - 1;      // 1024 threads a row, below 2^32 in a launch
 constexpr int kMaxCols = 1 << 30;
@@ -34,6 +35,10 @@ template <> struct Vec<float> {
   static constexpr int V = 4;
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ float get(const u32x4_t& r, int i) { return __uint_as_float(r[i]); }
+  static __device__ __forceinline__ float pick(const u32x4_t& r, int i) {     // i not known at compile time
+    const unsigned a = i & 1 ? r[1] : r[0], b = i & 1 ? r[3] : r[2];
+    return __uint_as_float(i & 2 ? b : a);
+  }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
   static __device__ __forceinline__ void putv(float* p, const float (&o)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{o[0], o[1], o[2], o[3]}; }
 };
@@ -42,6 +47,10 @@ template <> struct Vec<unsigned short> {
   static __device__ __forceinline__ float one(const unsigned short* p) { return bf16_to_f32(*p); }
   static __device__ __forceinline__ float get(const u32x4_t& r, int i) {
     return __uint_as_float(i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
+  }
+  static __device__ __forceinline__ float pick(const u32x4_t& r, int i) {
+    const unsigned a = i & 2 ? r[1] : r[0], b = i & 2 ? r[3] : r[2], w = i & 4 ? b : a;
+    return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
   }
   static __device__ __forceinline__ void put(unsigned short* p, float v) { *p = f32_to_bf16(v); }
   static __device__ __forceinline__ void putv(unsigned short* p, const float (&o)[8]) { store8_bf16(p, o); }
@@ -59,8 +68,9 @@ __device__ __forceinline__ float value_of(u64 key) {
   const unsigned o = (unsigned)(key >> 32);
   return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
 }
-__device__ __forceinline__ u64 shfl_u64(u64 v, int src) {
-  const unsigned lo = __shfl((int)(unsigned)v, src, 64), hi = __shfl((int)(unsigned)(v >> 32), src, 64);
+// lane src's value (src the same in every lane), without a trip through the LDS
+__device__ __forceinline__ u64 lane_u64(u64 v, int src) {
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)v, src), hi = __builtin_amdgcn_readlane((int)(unsigned)(v >> 32), src);
   return ((u64)hi << 32) | lo;
 }
 __device__ __forceinline__ u64 shfl_xor_u64(u64 v, int m) {
@@ -70,37 +80,36 @@ __device__ __forceinline__ u64 shfl_xor_u64(u64 v, int m) {
 
 struct Shared {
   u64 cand[kCap];
-  u64 best[kMaxTop];                 // the k best so far, descending; 0: none
+  u64 best[kMaxTop];                 // the k best so far, descending
+  u64 sorted[kMaxTop];
   u64 group[64];
   u64 threshold;
   int count;
   float red[3][16];
 };
 
-// The k best of best[] (nb of them) and cand[0 .. n), by counting the greater ones: one wave.
+// The k best of cand[0 .. n) and best[0 .. nb), by counting the greater ones: one wave.
 __device__ __forceinline__ void rank_candidates(Shared& sh, int n, int nb, int k, int lane) {
-  constexpr int M = (kCap + kMaxTop + 63) / 64;
-  u64 mine[M];
   const int total = n + nb;
-#pragma unroll
-  for (int c = 0; c < M; ++c) {
-    const int i = c * 64 + lane;
-    mine[c] = i < n ? sh.cand[i] : (i < total ? sh.best[i - n] : 0ull);
+  if (total <= 64) {                                     // almost always
+    const u64 mine = lane < n ? sh.cand[lane] : (lane < total ? sh.best[lane - n] : 0ull);
+    int rank = 0;
+    for (int j = 0; j < total; ++j) rank += lane_u64(mine, j) > mine ? 1 : 0;
+    if (lane < total && rank < k) sh.best[rank] = mine;
+    return;
   }
-  int rank[M] = {};
-  for (int j = 0; j < total; ++j) {
-    const u64 other = j < n ? sh.cand[j] : sh.best[j - n];
-#pragma unroll
-    for (int c = 0; c < M; ++c)
-      if (c * 64 < total) rank[c] += other > mine[c] ? 1 : 0;
+  for (int c = 0; c < total; c += 64) {
+    const int i = c + lane;
+    const u64 mine = i < n ? sh.cand[i] : (i < total ? sh.best[i - n] : 0ull);
+    int rank = 0;
+    for (int j = 0; j < total; ++j) rank += (j < n ? sh.cand[j] : sh.best[j - n]) > mine ? 1 : 0;
+    if (i < total && rank < k) sh.sorted[rank] = mine;
   }
-#pragma unroll
-  for (int c = 0; c < M; ++c)
-    if (c * 64 + lane < total && rank[c] < k) sh.best[rank[c]] = mine[c];
+  if (lane < (total < k ? total : k)) sh.best[lane] = sh.sorted[lane];
 }
 
 template <typename T, typename L, int NT, bool TOP>
-__global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict__ x, const L* __restrict__ tokens,
+__global__ __launch_bounds__(NT, 6) void token_logp_fwd_kernel(const T* __restrict__ x, const L* __restrict__ tokens,
                                                             float* __restrict__ logp, float* __restrict__ entropy,
                                                             float* __restrict__ top_logp, long long* __restrict__ top_ids,
                                                             float* __restrict__ stat, int N, int C, long long ld, int k) {
@@ -118,7 +127,7 @@ __global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict_
   const float xo = odd >= 0 ? Vec<T>::one(xr + odd) : -INFINITY;
 
   float m = -INFINITY, s = 0.f, w = 0.f;
-  int nb = 0;                                            // entries of sh.best
+  int nb = 0, held = 0;                                  // entries of sh.best; candidates of earlier chunks not ranked yet
   u64 threshold = 0;
   if (TOP && tid == 0) sh.count = 0;
   if (TOP) __syncthreads();
@@ -161,7 +170,7 @@ __global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict_
       }
     if (!TOP) continue;
 
-    const bool some = in[0] || (base == 0 && odd >= 0);
+    const bool some = in[0] || (base == 0 && odd >= 0);      // (chunks are filled from the front)
     if (base == 0) {
       // first threshold: k-th largest of 64 maxima. The index in a thread's key is that of its first element where this
       // is the maximum, otherwise its last one's: no element with the maximum has a lower key. An empty group has key 0
@@ -182,7 +191,7 @@ __global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict_
         const u64 mine = sh.group[lane];
         int rank = 0;
         for (int j = 0; j < 64; ++j) {
-          const u64 other = shfl_u64(mine, j);
+          const u64 other = lane_u64(mine, j);
           rank += other > mine || (other == mine && j < lane) ? 1 : 0;
         }
         if (rank == k - 1) sh.threshold = mine;
@@ -195,29 +204,41 @@ __global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict_
       // threshold 0: everything passes (value_of(0) is a NaN, which no element is below)
       const bool scan = some && (!(cm < tv) || s != s);
       auto offer = [&](float v, int index) {
-        if (v < tv) return;
         const u64 key = key_of(v, index);
         if (key < threshold) return;
         const int at = atomicAdd(&sh.count, 1);
         if (at < kCap) sh.cand[at] = key;
       };
       if (scan) {
-        if (base == 0 && odd >= 0) offer(xo, odd);
+        if (base == 0 && odd >= 0 && !(xo < tv)) offer(xo, odd);
 #pragma unroll
         for (int u = 0; u < kU; ++u)
           if (in[u]) {
-            const int first = head + (base + u * NT + tid) * V;
+            // the elements are converted again, not kept in 32 registers from the sums above
+            asm volatile("" : "+v"(r[u]));
+            unsigned pass = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) offer(Vec<T>::get(r[u], i), first + i);
+            for (int i = 0; i < V; ++i) pass |= Vec<T>::get(r[u], i) < tv ? 0u : 1u << i;
+            while (pass) {
+              const int i = __builtin_ctz(pass);
+              pass &= pass - 1;
+              offer(Vec<T>::pick(r[u], i), head + (base + u * NT + tid) * V + i);
+            }
           }
       }
       __syncthreads();
       const int count = sh.count;
       __syncthreads();                                   // (the next chunk counts on)
-      if (count == 0) break;
+      // ranked when they no longer fit a wave, and at the row's end
+      if (count <= kKeep && base + NT * kU < nvec) {
+        held = count;
+        break;
+      }
       if (count <= kCap) {
         if (wid == 0) rank_candidates(sh, count, nb, k, lane);
         nb = min(nb + count, k);
+        held = 0;
+        if (base + NT * kU >= nvec) break;
         __syncthreads();
         if (nb == k) threshold = sh.best[k - 1] + 1;     // later elements have to beat the k-th
         if (tid == 0) sh.count = 0;
@@ -225,16 +246,17 @@ __global__ __launch_bounds__(NT) void token_logp_fwd_kernel(const T* __restrict_
         break;
       }
       // too many (whole ranges of equal or ordered values): the k-th best of those held is a higher threshold that k
-      // elements still reach. Take the chunk again with it; at least kCap - k candidates fall away each time
-      u64 kept = lane < nb ? sh.best[lane] : 0ull;       // (every wave saves the list; one writes it back)
+      // elements still reach. Take the chunk again with it; at least kCap - kKeep - k candidates fall away each time.
+      // Those held from earlier chunks stay, before the ones that come again
+      if (wid == 0) {
+        const u64 kept = lane < nb ? sh.best[lane] : 0ull;
+        rank_candidates(sh, kCap, nb, k, lane);
+        if (lane == 0) sh.threshold = sh.best[k - 1];
+        if (lane < nb) sh.best[lane] = kept;
+        if (lane == 0) sh.count = held;
+      }
       __syncthreads();
-      if (wid == 0) rank_candidates(sh, kCap, nb, k, lane);
-      __syncthreads();
-      threshold = sh.best[k - 1];
-      __syncthreads();
-      if (wid == 0 && lane < nb) sh.best[lane] = kept;
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
+      threshold = sh.threshold;
     }
   }
 
@@ -339,6 +361,9 @@ __global__ __launch_bounds__(NT) void token_logp_bwd_kernel(const T* __restrict_
   }
 }
 
+// 1024 threads a row where the rows are too few to fill the CUs, else 256 (less waiting at a barrier)
+bool wide_rows(int N, int C) { return C > 4096 && N < 512; }
+
 }  // namespace
 
 // x [N, C] (row stride ld >= C; 0 fp32, 1 bf16), tokens [N] (0 int32, 1 int64; outside [0, C): logp 0), 0 <= k <= 32, k <= C.
@@ -348,11 +373,12 @@ DTF_API int dtf_token_logp_fwd(const void* x, const void* tokens, float* logp, f
                                int label_dtype, hipStream_t stream) {
   if (N <= 0) return 0;
   if (C <= 0 || ld < C || k < 0 || k > kMaxTop || k > C || N > kMaxRows || C > kMaxCols) return -1;
+  const bool wide = wide_rows(N, C);
 #define FWD(T, L, NT, TOP)                                                                                            \
   hipLaunchKernelGGL((token_logp_fwd_kernel<T, L, NT, TOP>), dim3(N), dim3(NT), 0, stream, (const T*)x, (const L*)tokens, \
                      logp, entropy, top_logp, top_ids, stat, N, C, ld, k)
 #define FWD_L(T, L) \
-  if (C > 8192) { if (k) FWD(T, L, 1024, true); else FWD(T, L, 1024, false); } else { if (k) FWD(T, L, 256, true); else FWD(T, L, 256, false); }
+  if (wide) { if (k) FWD(T, L, 1024, true); else FWD(T, L, 1024, false); } else { if (k) FWD(T, L, 256, true); else FWD(T, L, 256, false); }
   if (x_dtype == 0 && label_dtype == 0) { FWD_L(float, int) }
   else if (x_dtype == 0) { FWD_L(float, long long) }
   else if (label_dtype == 0) { FWD_L(unsigned short, int) }
@@ -370,10 +396,11 @@ DTF_API int dtf_token_logp_bwd(const void* x, const void* tokens, const float* s
   if (C <= 0 || ld < C || k < 0 || k > kMaxTop || k > C || N > kMaxRows || C > kMaxCols || (k && (!g_top || !top_ids)))
     return -1;
   if ((reinterpret_cast<uintptr_t>(x) & 15) != (reinterpret_cast<uintptr_t>(dx) & 15)) return -2;
+  const bool wide = wide_rows(N, C);
 #define BWD(T, L, NT)                                                                                                  \
   hipLaunchKernelGGL((token_logp_bwd_kernel<T, L, NT>), dim3(N), dim3(NT), 0, stream, (const T*)x, (const L*)tokens, stat, \
                      entropy, top_ids, g_logp, g_ent, g_top, (T*)dx, N, C, ld, k)
-#define BWD_L(T, L) if (C > 8192) BWD(T, L, 1024); else BWD(T, L, 256);
+#define BWD_L(T, L) if (wide) BWD(T, L, 1024); else BWD(T, L, 256);
   if (x_dtype == 0 && label_dtype == 0) { BWD_L(float, int) }
   else if (x_dtype == 0) { BWD_L(float, long long) }
   else if (label_dtype == 0) { BWD_L(unsigned short, int) }

@@ -98,7 +98,7 @@ class _BiasFn(torch.autograd.Function):
         d = torch.empty(shape, dtype=dt, device=g.device)
         w, n = _words(q_len, k_len, shape[1], q_start, d, max_distance, bidirectional)
         lib = _lib.kernels()
-        parts = torch.empty(lib.dtf_relative_bias_parts(q_len, k_len) * shape[0] * shape[1], dtype=torch.float32,
+        parts = torch.empty(lib.dtf_relative_bias_parts(q_len, k_len, shape[1]) * shape[0] * shape[1], dtype=torch.float32,
                             device=g.device)
         with _lib.on_device(g):
             rc = lib.dtf_relative_bias_bwd(w, n, _lib.ptr(g), _lib.ptr(parts), _lib.ptr(d), _lib.dtype_code(dt),
