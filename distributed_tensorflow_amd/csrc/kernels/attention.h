@@ -48,7 +48,8 @@ struct Args {
   float* stat;                       // [2][B, nh, Sq]: row maximum (in score units with biases, else base 2), log2 of the row sum
   float* delta;                      // [B, nh, Sq] rowsum(dO * O)
   float* dtab;                       // [B * query tiles][nh][buckets] partial sums of the table's gradient, or null
-  int B, Sq, Sk, nh, nkv, hd, causal;
+  float* part;                       // few queries: partial results of the key splits
+  int B, Sq, Sk, nh, nkv, hd, causal, splits;
   float scale;
 };
 
@@ -445,6 +446,266 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void fwd_kernel(Args
         a.stat[n + i] = lt == 0.f ? 0.f : flog2(lt);
       }
     }
+  }
+}
+
+// ================================================================================================== few queries
+// New tokens over a cache: at most 32 rows (queries x query heads of one key head), however many keys. Bound by the one
+// read of K and V, so the keys are split over workgroups until these fill the chip, each wave walks key tiles of its own
+// (32 keys, every fourth of its workgroup's), K goes from global memory straight into the product's operand, V through an
+// LDS image of the wave's own, and no barrier stands in the loop. All query heads of a key head ride in one tile of rows,
+// so the cache is read once, not once a query head. The waves' (maximum, sum, O) join in the LDS, the workgroups' in a
+// second kernel.
+constexpr int kFewRows = 32, kFewKeys = 32;
+
+// O and the row's statistics of row r of a key head's rows
+template <typename T, bool BIAS>
+__device__ __forceinline__ void few_store(const Args& a, int b, int kvh, int group, int r, int d, float mm, float lt,
+                                          const f32x4& acc, float c) {
+  const int i = r / group, h = kvh * group + r - i * group;
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  if (d < a.hd) store4((T*)a.out.p + b * a.out.sb + (long long)i * a.out.ss + h * a.out.sh + d, acc * inv);
+  if (d == 0 && a.stat) {
+    const long long at = ((long long)b * a.nh + h) * a.Sq + i, n = (long long)a.B * a.nh * a.Sq;
+    a.stat[at] = lt == 0.f ? INFINITY : (BIAS ? mm : mm * c);        // the units of fwd_kernel
+    a.stat[n + at] = lt == 0.f ? 0.f : flog2(lt);
+  }
+}
+
+template <typename T, int D, int QB, bool BIAS>
+__global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
+  constexpr int DB = D / 16, DS = D / 32, ST = row_stride<T, D>(), IMG = kFewKeys * ST, JOIN = QB * 16 * (D + 4) * 4;
+  constexpr int kChunk = 16 / (int)sizeof(T), kPerRow = D / kChunk, NV = kFewKeys * kPerRow / 64;
+  extern __shared__ __attribute__((aligned(16))) char smem[];      // [4 waves][V image, then O], [4][2][rows], table
+  constexpr int REGION = IMG > JOIN ? IMG : JOIN;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, g = lane >> 4;
+  char* vimg = smem + wid * REGION;
+  float* ml = reinterpret_cast<float*>(smem + 4 * REGION);
+  float* tab = ml + 4 * 2 * QB * 16;
+  const int group = a.nh / a.nkv, rows = a.Sq * group;
+  const int split = blockIdx.x % a.splits, bk = blockIdx.x / a.splits, b = bk / a.nkv, kvh = bk - b * a.nkv;
+  const int klen = a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk;
+  const int start = a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0;
+  const float c = a.scale * kLog2e;
+  const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
+  const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
+  const float* kbp = BIAS && a.key_bias ? a.key_bias + (long long)b * a.Sk : nullptr;
+
+  if (BIAS && a.table) {
+    for (int i = tid; i < group * a.buckets; i += 256) {
+      const int hg = i / a.buckets;
+      tab[i] = to_score_units(a, table_at(a, i - hg * a.buckets, kvh * group + hg));
+    }
+    __syncthreads();
+  }
+  Frag<T> qf[QB][DS];
+  int pos[QB];
+  const float* tb[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = min(qb * 16 + fr, rows - 1), i = r / group, hg = r - i * group;
+    const T* row = (const T*)a.q.p + b * a.q.sb + (long long)i * a.q.ss + (kvh * group + hg) * a.q.sh;
+    pos[qb] = start + i;
+    tb[qb] = tab + hg * a.buckets;
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks) frag_global(qf[qb][ks], row, ks * 32 + g * 8, ks * 32 + g * 8 < a.hd);
+  }
+  f32x4 o[DB][QB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m[QB], l[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) { m[qb] = -INFINITY; l[qb] = 0.f; }
+
+  const int kend = a.causal ? min(klen, start + a.Sq) : klen;
+  const int nt = kend > 0 ? (kend + kFewKeys - 1) / kFewKeys : 0, per = (nt + a.splits - 1) / a.splits;
+  const int t1 = min(nt, (split + 1) * per);
+
+  Frag<T> kf[2][DS];
+  u32x4_t vr[NV];
+  float kbv[NV];
+  f32x4 kb[2];
+  const unsigned kld = (unsigned)a.k.ss * (unsigned)sizeof(T), vld = (unsigned)a.v.ss * (unsigned)sizeof(T);
+  auto rsrc = [&](const T* base, unsigned ld, int left) {
+    left = min(left, kFewKeys);
+    const unsigned bytes = (unsigned)(left - 1) * ld + (unsigned)a.hd * (unsigned)sizeof(T);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+  };
+  auto fetch = [&](int t) {                              // (left >= 1: the tile starts before kend)
+    const int k0 = t * kFewKeys, left = klen - k0;
+    const __amdgpu_buffer_rsrc_t kr = rsrc(kp + (long long)k0 * a.k.ss, kld, left), vs = rsrc(vp + (long long)k0 * a.v.ss, vld, left);
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb) {
+      const int row = jb * 16 + fr;
+      const bool in = row < left && !(BIAS && kbp && kbp[k0 + row] == -INFINITY);
+#pragma unroll
+      for (int ks = 0; ks < DS; ++ks) {
+        const int e = ks * 32 + g * 8;
+        const unsigned off = in && e < a.hd ? (unsigned)row * kld + (unsigned)e * (unsigned)sizeof(T) : 0xffffffffu;
+        u32x4_t w[sizeof(Frag<T>) / 16];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(Frag<T>) / 16; ++i)
+          w[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(off == 0xffffffffu ? off : off + 16u * i), 0, 0));
+        __builtin_memcpy(&kf[jb][ks], w, sizeof(Frag<T>));
+      }
+      if (BIAS && kbp) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int k = k0 + jb * 16 + 4 * g + r;
+          kb[jb][r] = k < klen ? to_score_units(a, kbp[k]) : -INFINITY;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int p = u * 64 + lane, row = p / kPerRow, ch = p - row * kPerRow;
+      const bool in = row < left && ch * kChunk < a.hd && !(BIAS && kbp && kbp[k0 + row] == -INFINITY);
+      vr[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vs, (int)(in ? (unsigned)row * vld + (unsigned)ch * 16u : 0xffffffffu), 0, 0));
+    }
+  };
+
+  int t = split * per + wid;
+  if (t < t1) fetch(t);
+  for (; t < t1; t += 4) {
+    const int kt = t * kFewKeys;
+    f32x4 s[2][QB];
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        s[jb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (BIAS && kbp) s[jb][qb] = kb[jb];
+        if (BIAS && a.table) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[jb][qb][r] += tb[qb][bucket_of(a, kt + jb * 16 + 4 * g + r - pos[qb])];
+        }
+      }
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) s[jb][qb] = mma(kf[jb][ks], qf[qb][ks], s[jb][qb]);
+    // V of this tile to the LDS, the next tile's loads on their way (the LDS serves a wave in order: no barrier)
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int p = u * 64 + lane, row = p / kPerRow, ch = p - row * kPerRow;
+      *reinterpret_cast<u32x4_t*>(vimg + row * ST + ch * 16) = vr[u];
+    }
+    if (t + 4 < t1) fetch(t + 4);
+    Frag<T> pf[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const int end = a.causal ? min(klen, pos[qb] + 1) : klen;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (kt + jb * 16 + 4 * g + r >= end) s[jb][qb][r] = -INFINITY;
+          mx = fmaxf(mx, s[jb][qb][r]);
+        }
+      const float mn = fmaxf(m[qb], group_max(mx)), ref = mn == -INFINITY ? 0.f : mn;
+      const float alpha = fexp2((m[qb] - ref) * c);
+      m[qb] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[jb][qb][r] = fexp2((s[jb][qb][r] - ref) * c);
+          sum += s[jb][qb][r];
+        }
+      l[qb] = l[qb] * alpha + sum;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
+      pack(pf[qb], s[0][qb], s[1][qb]);
+    }
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      Frag<T> vf;
+      frag_tr<ST>(vf, vimg, db * 16, 0, lane);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) o[db][qb] = mma(vf, pf[qb], o[db][qb]);
+    }
+    asm volatile("" ::: "memory");
+  }
+  // join the waves
+  float* om = reinterpret_cast<float*>(vimg);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    l[qb] = group_sum(l[qb]);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(om + (qb * 16 + fr) * (D + 4) + db * 16 + g * 4) = o[db][qb];
+    if (g == 0) {
+      ml[(wid * 2 + 0) * QB * 16 + qb * 16 + fr] = m[qb];
+      ml[(wid * 2 + 1) * QB * 16 + qb * 16 + fr] = l[qb];
+    }
+  }
+  __syncthreads();
+  const long long n_rows = (long long)a.B * a.nkv * rows;
+  for (int p = tid; p < rows * (D / 4); p += 256) {
+    const int r = p / (D / 4), d = (p - r * (D / 4)) * 4;
+    float mm = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w * 2 * QB * 16 + r]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = fexp2((ml[w * 2 * QB * 16 + r] - ref) * c);
+      lt += f * ml[(w * 2 + 1) * QB * 16 + r];
+      acc += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem + w * REGION) + r * (D + 4) + d);
+    }
+    const long long row = (long long)bk * rows + r;
+    if (a.splits > 1) {
+      // [split][row][D] of O over the split's own sum and maximum, then [split][2][row] of these
+      if (d < a.hd) *reinterpret_cast<f32x4*>(a.part + ((long long)split * n_rows + row) * D + d) = acc;
+      float* st = a.part + (long long)a.splits * n_rows * D + (long long)split * 2 * n_rows;
+      if (d == 0) { st[row] = mm; st[n_rows + row] = lt; }
+    } else {
+      few_store<T, BIAS>(a, b, kvh, group, r, d, mm, lt, acc, c);
+    }
+  }
+}
+
+// One workgroup a row: its threads share out the row's splits as well as its elements, so that no thread waits for more
+// than a few loads one after the other (one wave a row, walking the splits: 13.5 us where few_kernel itself takes 12).
+template <typename T, int D, bool BIAS>
+__global__ __launch_bounds__(256) void few_join_kernel(Args a) {
+  constexpr int L = D / 4, S = 256 / L;                  // lanes of a row, splits taken at a time
+  __shared__ __attribute__((aligned(16))) float red[S][D + 4];
+  __shared__ float fac[64], stats[2];
+  const int group = a.nh / a.nkv, rows = a.Sq * group, tid = threadIdx.x;
+  const long long row = blockIdx.x, n_rows = gridDim.x;
+  const float c = a.scale * kLog2e;
+  const float* st = a.part + (long long)a.splits * n_rows * D;
+  const int sub = tid / L, d = (tid - sub * L) * 4;
+  if (tid < 64) {                                        // (at most 64 splits)
+    const bool in = tid < a.splits;
+    const float ms = in ? st[(long long)tid * 2 * n_rows + row] : -INFINITY;
+    const float ls = in ? st[(long long)tid * 2 * n_rows + n_rows + row] : 0.f;
+    const float mm = wave_max(ms), f = fexp2((ms - (mm == -INFINITY ? 0.f : mm)) * c);
+    const float lt = wave_sum(f * ls);
+    fac[tid] = f;
+    if (tid == 0) { stats[0] = mm; stats[1] = lt; }
+  }
+  __syncthreads();
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (sub < S && d < a.hd)
+    for (int s = sub; s < a.splits; s += S)
+      acc += fac[s] * *reinterpret_cast<const f32x4*>(a.part + ((long long)s * n_rows + row) * D + d);
+  if (sub < S) *reinterpret_cast<f32x4*>(&red[sub][d]) = acc;
+  __syncthreads();
+  if (sub == 0) {
+    for (int s = 1; s < S && s < a.splits; ++s) acc += *reinterpret_cast<const f32x4*>(&red[s][d]);
+    const int bk = (int)(row / rows), b = bk / a.nkv;
+    few_store<T, BIAS>(a, b, bk - b * a.nkv, group, (int)(row - (long long)bk * rows), d, stats[0], stats[1], acc, c);
   }
 }
 
@@ -964,9 +1225,32 @@ inline int launch(K kernel, long long blocks, int lds, const Args& a, hipStream_
   return (int)hipGetLastError();
 }
 
+// Key splits of the few-queries path: two workgroups a CU, and at least two key tiles for each of a workgroup's waves
+// (fewer and the joining costs more than the splitting gains). 1: no second kernel.
+inline bool few_queries(int Sq, int nh, int nkv) { return (long long)Sq * (nh / nkv) <= kFewRows; }
+inline int few_splits(int B, int Sk, int nkv) {
+  const long long groups = (long long)B * nkv, most = (Sk + 8 * kFewKeys - 1) / (8 * kFewKeys);
+  long long n = (512 + groups - 1) / groups;
+  n = n < most ? n : most;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+template <typename T, int D, int QB, bool BIAS>
+int run_few(const Args& a, hipStream_t stream) {
+  constexpr int img = kFewKeys * row_stride<T, D>(), join = QB * 16 * (D + 4) * 4;
+  const int lds = 4 * (img > join ? img : join) + 4 * (8 * QB * 16 + (a.table ? a.nh / a.nkv * a.buckets : 0));
+  const int rc = launch(few_kernel<T, D, QB, BIAS>, (long long)a.B * a.nkv * a.splits, lds, a, stream);
+  if (rc || a.splits == 1) return rc;
+  hipLaunchKernelGGL((few_join_kernel<T, D, BIAS>), dim3((unsigned)(a.B * a.nh * a.Sq)), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
 template <typename T, int D>
 int run_fwd(const Args& a, hipStream_t stream) {
   const bool bias = a.key_bias || a.table;
+  if (few_queries(a.Sq, a.nh, a.nkv)) {
+    if (a.Sq * (a.nh / a.nkv) <= 16) return bias ? run_few<T, D, 1, true>(a, stream) : run_few<T, D, 1, false>(a, stream);
+    return bias ? run_few<T, D, 2, true>(a, stream) : run_few<T, D, 2, false>(a, stream);
+  }
   const int nqt = (a.Sq + kRows - 1) / kRows, kt = key_tile<T>();
   const int band = a.table ? a.max_dist + a.right + 1 + 2 * kMargin : 0;
   const int lds = lds_tiles(sizeof(T), D) + 4 * (2 * kt + band);

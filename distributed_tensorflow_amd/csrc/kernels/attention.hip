@@ -9,20 +9,19 @@ using namespace dtf;
 namespace {
 
 enum Word {
-  kPtr = 0,              // q k v out dout dq dk dv
-  kStride = 8,           // (batch, token, head) strides of the eight, in elements
+  kTensors = 0,          // q k v out dout dq dk dv: pointer and (batch, token, head) strides in elements, four words each
   kKeyBias = 32, kLens, kQStart, kQStart0, kTable, kTableBf16, kBuckets, kMaxDist, kBidirectional,
-  kStat, kDelta, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kThr   // then the bucket borders
+  kStat, kDelta, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kPart, kThr   // then the bucket borders
 };
 
 bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   if (n_words < kThr) return false;
   attn::Strided* t[8] = {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv};
   for (int i = 0; i < 8; ++i) {
-    t[i]->p = (void*)w[kPtr + i];
-    t[i]->sb = w[kStride + 3 * i];
-    t[i]->ss = w[kStride + 3 * i + 1];
-    t[i]->sh = w[kStride + 3 * i + 2];
+    t[i]->p = (void*)w[kTensors + 4 * i];
+    t[i]->sb = w[kTensors + 4 * i + 1];
+    t[i]->ss = w[kTensors + 4 * i + 2];
+    t[i]->sh = w[kTensors + 4 * i + 3];
   }
   a.key_bias = (const float*)w[kKeyBias];
   a.lens = (const int*)w[kLens];
@@ -97,12 +96,21 @@ __global__ __launch_bounds__(256) void dtab_finish_kernel(const float* __restric
 
 }  // namespace
 
+// Key splits of the forward pass. More than one: it needs a scratch of splits * B * nh * Sq * (hd rounded up to 32, + 2)
+// floats.
+DTF_API int dtf_attention_splits(int B, int Sq, int Sk, int nh, int nkv) {
+  return nkv > 0 && attn::few_queries(Sq, nh, nkv) ? attn::few_splits(B, Sk, nkv) : 1;
+}
+
 DTF_API int dtf_attention_fwd(const long long* words, int n_words, float scale, hipStream_t stream) {
   attn::Args a = {};
   if (!unpack(words, n_words, scale, a)) return -1;
   const bool bf16 = words[kBf16];
   if (!operands_ok(a, bf16 ? 2 : 4, false)) return -2;
   if (!grid_ok(a)) return -3;
+  a.splits = dtf_attention_splits(a.B, a.Sq, a.Sk, a.nh, a.nkv);
+  a.part = (float*)words[kPart];
+  if (a.splits > 1 && !a.part) return -5;
   return bf16 ? attn::fwd_bf16(a, stream) : attn::fwd_f32(a, stream);
 }
 

@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 
 import torch
 
@@ -149,52 +150,97 @@ class _AttnFn(torch.autograd.Function):
 
 # ---------------------------------------------------------------------------------------- general attention
 # csrc/kernels/attention.h: any lengths, causal, grouped key / value heads, padded batches, strided operands, relative
-# position bias; bf16 and fp32. The words below are the enum of csrc/kernels/attention.hip.
-def _strides(t: torch.Tensor) -> tuple[int, int, int]:
-    """(batch, token, head) strides; those of axes of one element, which torch leaves arbitrary, as in a dense tensor."""
-    (B, S, n, hd), (sb, ss, sh, _) = t.shape, t.stride()
-    return (sb if B > 1 else 0), (ss if S > 1 else n * hd), (sh if n > 1 else 0)
+# position bias; bf16 and fp32. A call is an array of 64-bit words, the enum of csrc/kernels/attention.hip: four for each
+# of q, k, v, out, dout, dq, dk, dv (pointer; batch, token and head stride), then the rest.
+_NONE = (0, 0, 0, 0)
+_entry: dict = {}
 
 
-def _usable(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a dense copy of it when the kernels cannot address it in place: they read 16 bytes at a time along the
-    head, rows must not overlap, and a tile's offsets are 32-bit."""
-    per16 = 16 // t.element_size()
-    sb, ss, sh = _strides(t)
-    if (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and not (sb % per16 or ss % per16 or sh % per16) \
-            and t.shape[3] <= ss <= 1 << 22:
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
-
-
-def _words(ptrs, B, Sq, Sk, nh, nkv, hd, opts, key_bias, lens, starts, table, stat, delta=0, parts=0, dtable=0):
-    """``ptrs``: (pointer, strides) of q, k, v, out, dout, dq, dk, dv; ``None`` for those a pass has not."""
-    causal, _, start0, max_distance, bidirectional = opts
-    w = [0 if t is None else t[0] for t in ptrs]
-    for t in ptrs:
-        w += (0, 0, 0) if t is None else t[1]
-    borders = ()
-    if table is not None:
-        borders = _rel.bucket_borders(table.shape[0], max_distance, bidirectional)
-    w += (0 if key_bias is None else key_bias.data_ptr(), 0 if lens is None else lens.data_ptr(),
-          0 if starts is None else starts.data_ptr(), start0, 0 if table is None else table.data_ptr(),
-          int(table is not None and table.dtype == torch.bfloat16), 0 if table is None else table.shape[0], max_distance,
-          int(bidirectional), stat.data_ptr(), delta, parts, dtable, B, Sq, Sk, nh, nkv, hd, int(causal))
-    return w, borders
-
-
-def _call(name, w, borders, bf16, scale, like):
-    w = [*w, int(bf16), *borders]
+def _call(name: str, words, scale: float, like: torch.Tensor) -> None:
+    fn = _entry.get(name)
+    if fn is None:
+        fn = getattr(_lib.kernels(), name)
+        fn.argtypes = (ctypes.c_char_p, ctypes.c_int, ctypes.c_float, ctypes.c_void_p)
+        _entry[name] = fn
+    n = len(words)
     with _lib.on_device(like):
-        rc = getattr(_lib.kernels(), name)((ctypes.c_longlong * len(w))(*w), len(w), ctypes.c_float(scale),
-                                           _lib.stream_ptr(like.device))
-    _lib.check(rc, name)
+        rc = fn(struct.pack(f"{n}q", *words), n, scale, _lib.stream_ptr(like.device))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _view(t: torch.Tensor, first: int, heads: int):
-    """(pointer, strides) of ``heads`` heads of ``t`` from ``first`` on."""
-    st = _strides(t)
-    return t.data_ptr() + first * t.stride(2) * t.element_size(), st
+def _address(t: torch.Tensor):
+    """The four words of ``t``, or ``None`` when the kernels cannot address it in place: they read 16 bytes at a time
+    along the head, rows must not overlap, and a tile's offsets are 32-bit. The strides of axes of one element, which torch
+    leaves arbitrary, are those of a dense tensor."""
+    B, S, n, hd = t.shape
+    sb, ss, sh, se = t.stride()
+    if B == 1:
+        sb = 0
+    if S == 1:
+        ss = n * hd
+    if n == 1:
+        sh = 0
+    p = t.data_ptr()
+    if se != 1 or not hd <= ss <= 1 << 22 or (p | (sb | ss | sh) * t.element_size()) & 15:
+        return None
+    return p, sb, ss, sh
+
+
+def _usable(t: torch.Tensor):
+    """(tensor, address): ``t`` itself or a dense copy."""
+    w = _address(t)
+    if w is None:
+        t = t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+        w = _address(t)
+    return t, w
+
+
+def _heads(t: torch.Tensor, w, nh: int, nkv: int):
+    """The words of the query, key and value heads of a fused buffer."""
+    p, sb, ss, sh = w
+    step = t.stride(2) * t.element_size()
+    return p, sb, ss, sh, p + nh * step, sb, ss, sh, p + (nh + nkv) * step, sb, ss, sh
+
+
+def _dense(p, S, n, hd):
+    return p, S * n * hd, n * hd, hd
+
+
+def _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat):
+    """(out, q, k, v as the kernels read them, table, words of the call)."""
+    causal, scale, start0, max_distance, bidirectional = opts
+    q, qw = _usable(q)
+    B, Sq, nh, hd = q.shape
+    if k is None:
+        nh -= 2 * nkv
+        Sk = Sq
+        ins = _heads(q, qw, nh, nkv)
+    else:
+        (k, kw), (v, vw) = _usable(k), _usable(v)
+        Sk = k.shape[1]
+        ins = (*qw, *kw, *vw)
+    out = torch.empty(B, Sq, nh, hd, dtype=q.dtype, device=q.device)
+    bf16, rel, borders = int(q.dtype == torch.bfloat16), (0, 0, 0), ()
+    if table is not None:
+        table = table.contiguous()
+        rel = (table.data_ptr(), int(table.dtype == torch.bfloat16), table.shape[0])
+        borders = _rel.bucket_borders(table.shape[0], max_distance, bidirectional)
+    part, splits = 0, 1
+    if Sq * nh <= 32 * nkv and Sk > 256:           # few queries: the keys may be split over workgroups
+        splits = _lib.kernels().dtf_attention_splits(B, Sq, Sk, nh, nkv)
+        if splits > 1:
+            part = torch.empty(splits * B * nh * Sq * (-(-hd // 32) * 32 + 2), dtype=torch.float32, device=q.device)
+    words = (*ins, *_dense(out.data_ptr(), Sq, nh, hd), *_NONE, *_NONE, *_NONE, *_NONE,
+             0 if key_bias is None else key_bias.data_ptr(), 0 if lens is None else lens.data_ptr(),
+             0 if starts is None else starts.data_ptr(), start0, *rel, max_distance, int(bidirectional),
+             0 if stat is None else stat.data_ptr(), 0, 0, 0, B, Sq, Sk, nh, nkv, hd, int(causal), bf16,
+             part.data_ptr() if splits > 1 else 0, *borders)
+    if Sk == 0:
+        out.zero_()
+    elif out.numel():
+        _call("dtf_attention_fwd", words, scale, q)
+    return out, q, k, v, table, words
 
 
 class _GeneralFn(torch.autograd.Function):
@@ -202,60 +248,43 @@ class _GeneralFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, key_bias, lens, starts, nkv, opts):
-        packed = k is None
-        q = _usable(q)
-        if packed:
-            B, Sq, n, hd = q.shape
-            Sk, nh = Sq, n - 2 * nkv
-            qkv = (_view(q, 0, nh), _view(q, nh, nkv), _view(q, nh + nkv, nkv))
-        else:
-            k, v = _usable(k), _usable(v)
-            B, Sq, nh, hd = q.shape
-            Sk = k.shape[1]
-            qkv = tuple((t.data_ptr(), _strides(t)) for t in (q, k, v))
-        out = torch.empty(B, Sq, nh, hd, dtype=q.dtype, device=q.device)
-        stat = torch.empty(2, B, nh, Sq, dtype=torch.float32, device=q.device)
-        ctx.meta = (B, Sq, Sk, nh, nkv, hd, packed, opts)
+        B, Sq, n = q.shape[:3]
+        stat = torch.empty(2, B, n - 2 * nkv if k is None else n, Sq, dtype=torch.float32, device=q.device)
         ctx.table_like = None if table is None else (table.shape, table.dtype)
-        table = None if table is None else table.contiguous()
+        out, q, k, v, table, ctx.words = _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat)
+        ctx.scale = opts[1]
+        # (the words point into these)
         ctx.save_for_backward(q, k, v, table, key_bias, lens, starts, out, stat)
-        if Sk == 0:
-            return out.zero_()
-        if out.numel():
-            w, borders = _words((*qkv, (out.data_ptr(), _strides(out)), None, None, None, None), B, Sq, Sk, nh, nkv, hd,
-                                opts, key_bias, lens, starts, table, stat)
-            _call("dtf_attention_fwd", w, borders, q.dtype == torch.bfloat16, opts[1], q)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, key_bias, lens, starts, out, stat = ctx.saved_tensors
-        B, Sq, Sk, nh, nkv, hd, packed, opts = ctx.meta
-        dev = q.device
-        if packed:
-            dq, dk, dv = torch.empty(B, Sq, nh + 2 * nkv, hd, dtype=q.dtype, device=dev), None, None
-            qkv = (_view(q, 0, nh), _view(q, nh, nkv), _view(q, nh + nkv, nkv))
-            grads = (_view(dq, 0, nh), _view(dq, nh, nkv), _view(dq, nh + nkv, nkv))
+        q, k, v, table, *_, out, _ = ctx.saved_tensors
+        words, dev, dt = ctx.words, q.device, q.dtype
+        B, Sq, Sk, nh, nkv, hd = words[45:51]
+        dq = torch.empty(q.shape, dtype=dt, device=dev)
+        dk = dv = dtable = None
+        if k is None:
+            grads = _heads(dq, _dense(dq.data_ptr(), Sq, nh + 2 * nkv, hd), nh, nkv)
         else:
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-            qkv = tuple((t.data_ptr(), _strides(t)) for t in (q, k, v))
-            grads = tuple((t.data_ptr(), _strides(t)) for t in (dq, dk, dv))
-        dtable = parts = None
+            dk, dv = torch.empty(k.shape, dtype=dt, device=dev), torch.empty(k.shape, dtype=dt, device=dev)
+            grads = (*_dense(dq.data_ptr(), Sq, nh, hd), *_dense(dk.data_ptr(), Sk, nkv, hd),
+                     *_dense(dv.data_ptr(), Sk, nkv, hd))
+        n = B * nh * Sq
         if table is not None and ctx.needs_input_grad[3]:
-            shape, dt = ctx.table_like
-            dtable = torch.empty(shape, dtype=dt, device=dev)
-        if out.numel() == 0 or Sk == 0:
-            return (dq.zero_(), None if packed else dk.zero_(), None if packed else dv.zero_(),
-                    None if dtable is None else dtable.zero_(), None, None, None, None, None)
-        if dtable is not None:
-            parts = torch.empty(B * (-(-Sq // 128)) * dtable.numel(), dtype=torch.float32, device=dev)
-        dout = _usable(dout)
-        delta = torch.empty(B, nh, Sq, dtype=torch.float32, device=dev)
-        w, borders = _words((*qkv, (out.data_ptr(), _strides(out)), (dout.data_ptr(), _strides(dout)), *grads), B, Sq, Sk,
-                            nh, nkv, hd, opts, key_bias, lens, starts, table, stat, delta.data_ptr(),
-                            0 if parts is None else parts.data_ptr(), 0 if dtable is None else dtable.data_ptr())
-        _call("dtf_attention_bwd", w, borders, q.dtype == torch.bfloat16, opts[1], q)
+            dtable = torch.empty(ctx.table_like[0], dtype=ctx.table_like[1], device=dev)
+        if n == 0 or Sk == 0:
+            for t in (dq, dk, dv, dtable):
+                if t is not None:
+                    t.zero_()
+            return dq, dk, dv, dtable, None, None, None, None, None
+        # rowsum(dO * O), then the partial sums of the table's gradient
+        scratch = torch.empty(n + (0 if dtable is None else B * -(-Sq // 128) * dtable.numel()), dtype=torch.float32, device=dev)
+        p = scratch.data_ptr()
+        dout, dw = _usable(dout)
+        _call("dtf_attention_bwd", (*words[:16], *dw, *grads, *words[32:42], p, *((0, 0) if dtable is None else
+              (p + 4 * n, dtable.data_ptr())), *words[45:]), ctx.scale, q)
         return dq, dk, dv, dtable, None, None, None, None, None
 
 
@@ -328,8 +357,12 @@ def _general(q, k, v, nkv, key_bias, causal, scale, key_lengths, q_start, rel_ta
         if rel_table.device != q.device:
             raise ValueError(f"rel_table is on {rel_table.device}, the queries on {q.device}")
     opts = (bool(causal), scale, start0, int(rel_max_distance), bidirectional)
-    run = _GeneralFn.apply if q.is_cuda else _composed
-    return run(q, k, v, rel_table, key_bias, lens, starts, nkv, opts)
+    if not q.is_cuda:
+        return _composed(q, k, v, rel_table, key_bias, lens, starts, nkv, opts)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad))
+                                    or (rel_table is not None and rel_table.requires_grad)):
+        return _GeneralFn.apply(q, k, v, rel_table, key_bias, lens, starts, nkv, opts)
+    return _forward(q, k, v, rel_table, key_bias, lens, starts, nkv, opts, None)[0]
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_bias: torch.Tensor | None = None, *,

@@ -17,7 +17,7 @@ exact^(half - exact)``), so a distance that lies on a border is not decided by r
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from functools import lru_cache
 
 import torch
@@ -67,41 +67,44 @@ def relative_bucket(distance: torch.Tensor, buckets: int, max_distance: int = 12
     return b + half * (d > 0) if bidirectional else b
 
 
-def _words(q_len: int, k_len: int, heads: int, q_start: int, table: torch.Tensor, max_distance: int, bidirectional: bool):
-    borders = bucket_borders(table.shape[0], max_distance, bidirectional)
-    w = (q_len, k_len, heads, q_start, table.shape[0], max_distance, int(bidirectional), *borders)
-    return (ctypes.c_longlong * len(w))(*w), len(w)
+def _words(q_len: int, k_len: int, heads: int, q_start: int, buckets: int, max_distance: int, bidirectional: bool):
+    w = (q_len, k_len, heads, q_start, buckets, max_distance, int(bidirectional),
+         *bucket_borders(buckets, max_distance, bidirectional))
+    return struct.pack(f"{len(w)}q", *w), len(w)
+
+
+def _forward(table, q_len, k_len, q_start, max_distance, bidirectional):
+    t = table.contiguous()
+    out = torch.empty(t.shape[1], q_len, k_len, dtype=t.dtype, device=t.device)
+    if out.numel():
+        w = _words(q_len, k_len, t.shape[1], q_start, t.shape[0], max_distance, bidirectional)
+        with _lib.on_device(t):
+            rc = _lib.kernels().dtf_relative_bias_fwd(*w, _lib.ptr(t), _lib.ptr(out), _lib.dtype_code(t.dtype),
+                                                      _lib.stream_ptr(t.device))
+        _lib.check(rc, "relative_bias_fwd")
+    return out
 
 
 class _BiasFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, q_len, k_len, q_start, max_distance, bidirectional):
-        t = table.contiguous()
-        heads = t.shape[1]
-        out = torch.empty(heads, q_len, k_len, dtype=t.dtype, device=t.device)
-        ctx.meta = (q_len, k_len, q_start, max_distance, bidirectional, t.shape, t.dtype)
-        if out.numel():
-            w, n = _words(q_len, k_len, heads, q_start, t, max_distance, bidirectional)
-            with _lib.on_device(t):
-                rc = _lib.kernels().dtf_relative_bias_fwd(w, n, _lib.ptr(t), _lib.ptr(out), _lib.dtype_code(t.dtype),
-                                                          _lib.stream_ptr(t.device))
-            _lib.check(rc, "relative_bias_fwd")
-        return out
+    def forward(ctx, table, *args):
+        ctx.meta = (*args, table.shape, table.dtype)
+        return _forward(table, *args)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         q_len, k_len, q_start, max_distance, bidirectional, shape, dt = ctx.meta
-        g = g.contiguous()
         if g.numel() == 0:
             return torch.zeros(shape, dtype=dt, device=g.device), None, None, None, None, None
+        g = g.contiguous()
         d = torch.empty(shape, dtype=dt, device=g.device)
-        w, n = _words(q_len, k_len, shape[1], q_start, d, max_distance, bidirectional)
         lib = _lib.kernels()
         parts = torch.empty(lib.dtf_relative_bias_parts(q_len, k_len, shape[1]) * shape[0] * shape[1], dtype=torch.float32,
                             device=g.device)
+        w = _words(q_len, k_len, shape[1], q_start, shape[0], max_distance, bidirectional)
         with _lib.on_device(g):
-            rc = lib.dtf_relative_bias_bwd(w, n, _lib.ptr(g), _lib.ptr(parts), _lib.ptr(d), _lib.dtype_code(dt),
+            rc = lib.dtf_relative_bias_bwd(*w, _lib.ptr(g), _lib.ptr(parts), _lib.ptr(d), _lib.dtype_code(dt),
                                            _lib.stream_ptr(g.device))
         _lib.check(rc, "relative_bias_bwd")
         return d, None, None, None, None, None
@@ -118,6 +121,7 @@ def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: 
     if q_len < 0 or k_len < 0 or max(q_len, k_len) > 1 << 28 or abs(q_start) > 1 << 29:
         raise ValueError(f"lengths {q_len} and {k_len} with the first query at {q_start} are out of range")
     if table.is_cuda:
-        return _BiasFn.apply(table, q_len, k_len, q_start, max_distance, bidirectional)
+        run = _BiasFn.apply if table.requires_grad and torch.is_grad_enabled() else _forward
+        return run(table, q_len, k_len, q_start, max_distance, bool(bidirectional))
     d = torch.arange(k_len)[None, :] - (torch.arange(q_len)[:, None] + q_start)
     return table.t()[:, relative_bucket(d, table.shape[0], max_distance, bidirectional)]
