@@ -46,20 +46,39 @@ struct Args {
   int table_bf16, buckets, half, exact, max_dist, right;   // right: max_dist when bidirectional, else 0
   int n_thr, thr[kMaxThr];           // thr[t]: smallest |distance| of bucket exact + 1 + t
   float* stat;                       // [2][B, nh, Sq]: row maximum (in score units with biases, else base 2), log2 of the row sum
-  float* delta;                      // [B, nh, Sq] rowsum(dO * O)
+  float* rows;                       // [B * nh][64-row tiles][4][64]: what the dK / dV kernel wants of each query, see kRowStats
   float* dtab;                       // [B * query tiles][nh][buckets] partial sums of the table's gradient, or null
-  float* part;                       // few queries: partial results of the key splits
-  int B, Sq, Sk, nh, nkv, hd, causal, splits;
-  float scale;
+  float* part;                       // partial results of the key splits (few queries), of the head splits (dK / dV)
+  int B, Sq, Sk, nh, nkv, hd, causal, splits, ksplits;
+  float scale, inv_scale;
 };
+
+// What the dK / dV kernel wants of each query, in tiles of 64 that one direct load of 1 KiB brings to the LDS: the row
+// maximum with log2 of the row sum added (with key biases: without, and that on its own) and -D; rows past the end have
+// the maximum +inf, that is probabilities 0. The dQ kernel writes them, for whole workgroups of 128 rows.
+constexpr int kRowStats = 256;       // floats of a tile: [maximum | log sum | -D | unused][64]
+__device__ __forceinline__ long long row_tile(const Args& a, long long bh, int tile) {
+  return (bh * ((a.Sq + kRows - 1) / kRows * 2) + tile) * kRowStats;
+}
 
 template <typename T> struct Frag;
 template <> struct Frag<unsigned short> { bf16x8_t v; };
 template <> struct Frag<float> { f32x4 lo, hi; };
 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
-// LDS row strides in bytes. +16: the 16 rows of a ds_read_b128 fragment start 4 banks apart (mod 64) for every D.
-template <typename T, int D> constexpr int row_stride() { return D * (int)sizeof(T) + 16; }
+// Tile images in the LDS. bf16: rows of 64, 128 or 256 bytes (head sizes over 64 take 256) without padding, as the direct
+// loads need them, their 16-byte chunks permuted by an XOR with swz(row). With 64 banks of 4 bytes the 16 rows of a
+// ds_read_b128 fragment then fall on different banks, and so do the 8 rows of half a transposing read, whose lanes take
+// 32 bytes of each (two chunks whose indices differ in bit 0): the rows that share a bank offset get different swz for
+// the first and different swz >> 1 for the second. fp32: padded by 16 bytes, which spreads its 16- and 4-byte reads.
+template <typename T, int D> constexpr int row_stride() {
+  return sizeof(T) == 4 ? D * 4 + 16 : (D == 32 ? 64 : D == 64 ? 128 : 256);
+}
+template <int STRIDE> __device__ __forceinline__ int swz(int row) {
+  if (STRIDE == 64) return ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+  if (STRIDE == 128) return ((row >> 1) & 3) << 1 | ((row >> 3) & 1);
+  return (row & 7) << 1 | ((row >> 3) & 1);
+}
 
 __device__ __forceinline__ f32x4 mma(const Frag<unsigned short>& a, const Frag<unsigned short>& b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
@@ -72,6 +91,13 @@ __device__ __forceinline__ f32x4 mma(const Frag<float>& a, const Frag<float>& b,
   return c;
 }
 
+// v, of which the compiler forgets where it came from
+__device__ __forceinline__ int opaque(int v) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(v));
+#endif
+  return v;
+}
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float flog2(float x) { return __builtin_amdgcn_logf(x); }
 
@@ -81,38 +107,69 @@ __device__ __forceinline__ void pack(Frag<unsigned short>& f, const f32x4& a, co
 }
 __device__ __forceinline__ void pack(Frag<float>& f, const f32x4& a, const f32x4& b) { f.lo = a; f.hi = b; }
 
-// 16 rows from row0 x 32 contraction elements ks of a tile image, 8 consecutive elements per lane
-template <int STRIDE>
-__device__ __forceinline__ void frag_row(Frag<unsigned short>& f, const char* img, int row0, int ks, int lane) {
-  f.v = *reinterpret_cast<const bf16x8_t*>(img + (row0 + (lane & 15)) * STRIDE + ks * 64 + (lane >> 4) * 16);
+// byte of a row's 16-byte chunk ch
+template <typename T, int D> __device__ __forceinline__ int chunk_at(int row, int ch) {
+  constexpr int S = row_stride<T, D>();
+  return row * S + ((sizeof(T) == 2 ? ch ^ swz<S>(row) : ch) << 4);
 }
-template <int STRIDE>
-__device__ __forceinline__ void frag_row(Frag<float>& f, const char* img, int row0, int ks, int lane) {
-  const char* p = img + (row0 + (lane & 15)) * STRIDE + ks * 128 + (lane >> 4) * 32;
-  f.lo = *reinterpret_cast<const f32x4*>(p);
-  f.hi = *reinterpret_cast<const f32x4*>(p + 16);
-}
-// the transposed product's operand: column c0 + (lane & 15) of the image, its 32 rows ks in the order of pack(): rows
-// 32 ks + 4 g .. +3, then 32 ks + 16 + 4 g .. +3 for lane group g
-template <int STRIDE>
-__device__ __forceinline__ void frag_tr(Frag<unsigned short>& f, const char* img, int c0, int ks, int lane) {
-  const int g = lane >> 4, t = lane & 15, q = t >> 2, p = t & 3;
-  const char* at = img + (ks * 32 + 4 * g + q) * STRIDE + c0 * 2 + p * 8;
-  typedef __attribute__((address_space(3))) s16x4_f* lp_t;
-  const s16x4_f lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp_t)at);
-  const s16x4_f hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp_t)(at + 16 * STRIDE));
-  const s16x8_f v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  f.v = __builtin_bit_cast(bf16x8_t, v);
-}
-template <int STRIDE>
-__device__ __forceinline__ void frag_tr(Frag<float>& f, const char* img, int c0, int ks, int lane) {
-  const char* at = img + (ks * 32 + 4 * (lane >> 4)) * STRIDE + (c0 + (lane & 15)) * 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f.lo[i] = *reinterpret_cast<const float*>(at + i * STRIDE);
-    f.hi[i] = *reinterpret_cast<const float*>(at + (16 + i) * STRIDE);
+
+// Reads of a tile image. Row: 16 rows from row0 x 32 contraction elements ks, 8 consecutive elements a lane. Tr: the
+// transposed product's operand, column c0 + (lane & 15) of the image, its 32 rows ks in the order of pack(): rows
+// 32 ks + 4 g .. +3, then 32 ks + 16 + 4 g .. +3 for lane group g. The lane's part of the addresses is computed once
+// (the swizzle sees only the low four bits of a row); row0 and ks of Tr are immediate offsets.
+template <typename T, int D, bool KEEP = true> struct Reader;
+template <int D, bool KEEP> struct Reader<unsigned short, D, KEEP> {
+  static constexpr int S = row_stride<unsigned short, D>();
+  static constexpr bool kKeep = KEEP;                    // false: no registers to spare, one XOR an access
+  int row[kKeep ? D / 32 : 1], tr[kKeep ? D / 16 : 1];
+  static __device__ __forceinline__ int flip(int at, int bits) {    // at ^ bits, which the compiler does not keep in a register
+    int o = 0;
+#ifdef __HIP_DEVICE_COMPILE__                            // (the host pass does not know the register class)
+    asm volatile("v_xor_b32 %0, %2, %1" : "=v"(o) : "v"(at), "i"(bits));
+#endif
+    return o;
   }
-}
+  __device__ __forceinline__ explicit Reader(int lane) {
+    const int fr = lane & 15, g = lane >> 4, q = fr >> 2, p = fr & 3, k = 4 * g + q;
+    const int row0 = fr * S + ((g ^ swz<S>(fr)) << 4), tr0 = k * S + (((p >> 1) ^ swz<S>(k)) << 4) + ((p & 1) << 3);
+#pragma unroll
+    for (int ks = 0; ks < (kKeep ? D / 32 : 1); ++ks) row[ks] = row0 ^ (ks << 6);
+#pragma unroll
+    for (int db = 0; db < (kKeep ? D / 16 : 1); ++db) tr[db] = tr0 ^ (db << 5);
+  }
+  __device__ __forceinline__ void read_row(Frag<unsigned short>& f, const char* img, int row0, int ks) const {
+    f.v = *reinterpret_cast<const bf16x8_t*>(img + (kKeep ? row[kKeep ? ks : 0] : flip(row[0], ks << 6)) + row0 * S);
+  }
+  __device__ __forceinline__ void read_tr(Frag<unsigned short>& f, const char* img, int db, int ks) const {
+    const char* at = img + (kKeep ? tr[kKeep ? db : 0] : flip(tr[0], db << 5)) + ks * 32 * S;
+    typedef __attribute__((address_space(3))) s16x4_f* lp_t;
+    const s16x4_f lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp_t)at);
+    const s16x4_f hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp_t)(at + 16 * S));
+    const s16x8_f v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    f.v = __builtin_bit_cast(bf16x8_t, v);
+  }
+};
+template <int D, bool KEEP> struct Reader<float, D, KEEP> {
+  static constexpr int S = row_stride<float, D>();
+  int row, tr;
+  __device__ __forceinline__ explicit Reader(int lane) {
+    row = (lane & 15) * S + (lane >> 4) * 32;
+    tr = 4 * (lane >> 4) * S + (lane & 15) * 4;
+  }
+  __device__ __forceinline__ void read_row(Frag<float>& f, const char* img, int row0, int ks) const {
+    const char* at = img + row + row0 * S + ks * 128;
+    f.lo = *reinterpret_cast<const f32x4*>(at);
+    f.hi = *reinterpret_cast<const f32x4*>(at + 16);
+  }
+  __device__ __forceinline__ void read_tr(Frag<float>& f, const char* img, int db, int ks) const {
+    const char* at = img + tr + ks * 32 * S + db * 64;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f.lo[i] = *reinterpret_cast<const float*>(at + i * S);
+      f.hi[i] = *reinterpret_cast<const float*>(at + (16 + i) * S);
+    }
+  }
+};
 
 // 8 consecutive elements of one row straight from global memory; zero beyond the head size
 __device__ __forceinline__ void frag_global(Frag<unsigned short>& f, const unsigned short* row, int e, bool ok) {
@@ -159,52 +216,94 @@ __device__ __forceinline__ float group_sum(float v) {
   return __uint_as_float(c) + __uint_as_float(d);
 }
 
-// Tile of ROWS rows x D elements between global memory and a padded LDS image, through registers. Rows from `left` on and
-// elements beyond the head size arrive as zeros: their addresses fail the buffer descriptor's range check. The
-// descriptor covers one tile only, so offsets stay 32-bit whatever the tensor's size.
-template <typename T, int D, int ROWS>
-struct Tile {
-  static constexpr int kChunk = 16 / (int)sizeof(T), kPerRow = D / kChunk, N = ROWS * kPerRow / 256;
+// A tile of ROWS rows x D elements from global memory to an LDS image, by 256 threads. Rows from `left` on and elements
+// beyond the head size arrive as zeros: their addresses fail the buffer descriptor's range check. The descriptor covers
+// one tile only, so offsets stay 32-bit whatever the tensor's size, and a lane's offsets are the same for every tile. A
+// key whose bias is -inf takes no part whatever K and V hold there: its row is read as zeros too.
+// bf16: loads that go to the LDS directly (64 lanes x 16 bytes fill 1 KiB in lane order; the swizzle is in the SOURCE
+// address). fp32: through registers, put() stores them.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, unsigned row_bytes, unsigned bytes_per_row_used, int left, int rows) {
+  left = left < 0 ? 0 : (left > rows ? rows : left);
+  const unsigned bytes = left ? (unsigned)(left - 1) * row_bytes + bytes_per_row_used : 0u;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+template <typename T, int D, int ROWS> struct Tile;
+template <int D, int ROWS>
+struct Tile<unsigned short, D, ROWS> {
+  static constexpr int S = row_stride<unsigned short, D>(), kSlots = S / 16, N = ROWS * S / 4096, IMG = ROWS * S;
+  const unsigned short* base;
+  unsigned ldb, used, off[N];
+  long long step;                                        // elements from tile to tile
+  int row[N];
+  __device__ __forceinline__ Tile(const unsigned short* p, long long ss, int hd, int tid) : base(p), step(ss * ROWS) {
+    ldb = (unsigned)ss * 2u;
+    used = (unsigned)hd * 2u;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int i = (u * 4 + (tid >> 6)) * 64 + (tid & 63);
+      row[u] = i / kSlots;
+      const int ch = (i % kSlots) ^ swz<S>(row[u]);
+      off[u] = ch * 8 < hd ? (unsigned)row[u] * ldb + (unsigned)ch * 16u : 0xffffffffu;
+    }
+  }
+  typedef __attribute__((address_space(3))) void* lds_t;
+  __device__ __forceinline__ void load(int t, int left, char* img, int wid) const {
+    const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base + t * step, ldb, used, left, ROWS);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(img + (u * 4 + wid) * 1024), 16, (int)off[u], 0, 0, 0);
+  }
+  __device__ __forceinline__ void load_masked(int t, int left, char* img, int wid, const float (&kb)[N]) const {
+    const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base + t * step, ldb, used, left, ROWS);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t)(img + (u * 4 + wid) * 1024), 16, kb[u] == -INFINITY ? -1 : (int)off[u], 0, 0, 0);
+  }
+  __device__ __forceinline__ void put(char*) const {}
+};
+template <int D, int ROWS>
+struct Tile<float, D, ROWS> {
+  static constexpr int S = row_stride<float, D>(), kPerRow = D / 4, N = ROWS * kPerRow / 256, IMG = ROWS * S;
+  const float* base;
+  unsigned ldb, used, off[N];
+  long long step;
+  int row[N], at[N];
   u32x4_t v[N];
-  float kb[N];
-
-  __device__ __forceinline__ void load(const T* base, long long ss, int left, int hd, int tid) {
-    left = left < 0 ? 0 : (left > ROWS ? ROWS : left);
-    const unsigned ldb = (unsigned)ss * (unsigned)sizeof(T);
-    const unsigned bytes = left ? (unsigned)(left - 1) * ldb + (unsigned)hd * (unsigned)sizeof(T) : 0u;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+  __device__ __forceinline__ Tile(const float* p, long long ss, int hd, int tid) : base(p), step(ss * ROWS) {
+    ldb = (unsigned)ss * 4u;
+    used = (unsigned)hd * 4u;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int p = u * 256 + tid, row = p / kPerRow, ch = p - row * kPerRow;
-      const bool ok = ch * kChunk < hd && row < left;
-      const unsigned off = ok ? (unsigned)row * ldb + (unsigned)ch * 16u : 0xffffffffu;
-      v[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
+      const int i = u * 256 + tid, ch = i % kPerRow;
+      row[u] = i / kPerRow;
+      at[u] = row[u] * S + ch * 16;
+      off[u] = ch * 4 < hd ? (unsigned)row[u] * ldb + (unsigned)ch * 16u : 0xffffffffu;
     }
   }
-  // keys whose bias is -inf take no part whatever K and V hold there: their rows are zeroed on the way to the LDS
-  __device__ __forceinline__ void load_bias(const float* bias, int left, int tid) {
+  __device__ __forceinline__ void load(int t, int left, char*, int) {
+    const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base + t * step, ldb, used, left, ROWS);
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int row = (u * 256 + tid) / kPerRow;
-      kb[u] = row < left ? bias[row] : 0.f;
-    }
+    for (int u = 0; u < N; ++u) v[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off[u], 0, 0));
   }
-  __device__ __forceinline__ void store(char* img, int tid) const {
+  __device__ __forceinline__ void load_masked(int t, int left, char*, int, const float (&kb)[N]) {
+    const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base + t * step, ldb, used, left, ROWS);
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int p = u * 256 + tid, row = p / kPerRow, ch = p - row * kPerRow;
-      *reinterpret_cast<u32x4_t*>(img + row * row_stride<T, D>() + ch * 16) = v[u];
-    }
+    for (int u = 0; u < N; ++u)
+      v[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, kb[u] == -INFINITY ? -1 : (int)off[u], 0, 0));
   }
-  __device__ __forceinline__ void store_masked(char* img, int tid) const {
-    const u32x4_t z = {0u, 0u, 0u, 0u};
+  __device__ __forceinline__ void put(char* img) const {
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int p = u * 256 + tid, row = p / kPerRow, ch = p - row * kPerRow;
-      *reinterpret_cast<u32x4_t*>(img + row * row_stride<T, D>() + ch * 16) = kb[u] == -INFINITY ? z : v[u];
-    }
+    for (int u = 0; u < N; ++u) *reinterpret_cast<u32x4_t*>(img + at[u]) = v[u];
   }
 };
+// the key biases of the rows of a tile that a thread loads
+template <int N>
+__device__ __forceinline__ void row_bias(float (&kb)[N], const int (&row)[N], const float* bias, int left) {
+#pragma unroll
+  for (int u = 0; u < N; ++u) kb[u] = row[u] < left ? bias[row[u]] : 0.f;
+}
+// the direct loads of this wave have arrived (the barrier after it makes that true for every wave's)
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- relative position bias ------------------------------------------------------------------------------------
 // The bias depends on the distance alone, and from max_dist on (right of the diagonal: `right`) it is one constant, so a
@@ -224,17 +323,27 @@ __device__ __forceinline__ float table_at(const Args& a, int bucket, int h) {
   const long long i = (long long)bucket * a.nh + h;
   return a.table_bf16 ? bf16_to_f32(((const unsigned short*)a.table)[i]) : ((const float*)a.table)[i];
 }
-// a finite bias stays finite in score units, and so does that times scale log2 e: it is never taken for a masked key
+// Biases in score units. A key bias is a mask as well: a finite one stays finite, and so does its product with
+// scale log2 e, so it is never taken for -inf. A learned value is held to +-2^24 powers of two (beyond that the scores
+// next to it would be lost in fp32 anyway), so that the kernels without key bias may take the maximum off by one fma.
 __device__ __forceinline__ float to_score_units(const Args& a, float bias) {
   const float lim = 3.0e38f / fmaxf(1.f, a.scale * kLog2e);
-  const float v = bias / a.scale;
+  const float v = bias * a.inv_scale;
   if (bias == -INFINITY) return bias;
   return v < -lim ? -lim : v;        // NaN and +inf pass
 }
+__device__ __forceinline__ float learned_bias(const Args& a, float bias) {
+  if (bias == -INFINITY || bias == INFINITY) return bias;
+  const float lim = 16777216.f / kLog2e, v = bias > lim ? lim : bias < -lim ? -lim : bias;
+  return v * a.inv_scale;
+}
 __device__ __forceinline__ void fill_band(const Args& a, int h, float* band, int tid) {
   const int n = band_size(a);
-  for (int i = tid; i < n; i += 256) band[i] = to_score_units(a, table_at(a, bucket_of(a, i - kMargin - a.max_dist), h));
+  for (int i = tid; i < n; i += 256) band[i] = learned_bias(a, table_at(a, bucket_of(a, i - kMargin - a.max_dist), h));
 }
+// What a kernel instance knows of the biases: none, the relative one alone, or a key bias with or without it.
+enum Mode { kPlain = 0, kRel = 1, kKeys = 2 };
+
 // the distances of bucket u, inclusive, clipped to the band
 __device__ __forceinline__ void bucket_range(const Args& a, int u, int& lo, int& hi) {
   const int lowest = -a.max_dist - kMargin, highest = a.right + kMargin;
@@ -262,28 +371,40 @@ __device__ __forceinline__ int xcd_contiguous(int bid, int n) {
   return x * q + (x < r ? x : r) + (bid >> 3);
 }
 
+// A value that is the same in every lane, in a scalar register (a quotient is computed in vector registers, and what is
+// derived from it stays there unless told)
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The i-th of n tiles of unequal work, w = 0 the longest: the first half longest first, then the other half shortest
+// first, so that two workgroups that come to one CU half a round apart add up to the same work.
+__device__ __forceinline__ int balanced(int i, int n) {
+  const int first = (n + 1) / 2;
+  return i < first ? i : n - 1 - (i - first);
+}
+
 // ================================================================================================== forward
-template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void fwd_kernel(Args a) {
-  constexpr int KT = key_tile<T>(), JB = KT / 16, DB = D / 16, DS = D / 32, ST = row_stride<T, D>(), IMG = KT * ST;
+template <typename T, int D, int MODE, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) : (D <= 64 ? 2 : GROUPS))) void fwd_kernel(Args a) {
+  constexpr int KT = key_tile<T>(), JB = KT / 16, DB = D / 16, DS = D / 32, IMG = Tile<T, D, KT>::IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V], [2][key bias of the tile], band
-  float* kbl = reinterpret_cast<float*>(smem + 4 * IMG);
-  float* band = kbl + 2 * KT;
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x & 255, lane = tid & 63, wid = uni(tid >> 6), grp = GROUPS > 1 ? uni(threadIdx.x >> 8) : 0;
+  char* mem = smem + grp * (4 * IMG + 8 * KT);                     // the group's tile images and key biases
+  float* kbl = reinterpret_cast<float*>(mem + 4 * IMG);
+  float* band = reinterpret_cast<float*>(smem + GROUPS * (4 * IMG + 8 * KT));
   const int fr = lane & 15, g = lane >> 4;
   const int nqt = (a.Sq + kRows - 1) / kRows;
-  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int qt = a.causal ? nqt - 1 - id % nqt : id % nqt, bh = id / nqt, b = bh / a.nh, h = bh - b * a.nh;
-  const int kvh = h / (a.nh / a.nkv);
+  const int id = uni(xcd_contiguous(blockIdx.x, gridDim.x));
+  const int bh = uni(id / nqt), ix = id - bh * nqt, b = uni(bh / a.nh), h = bh - b * a.nh;
+  const int qt = a.causal ? nqt - 1 - balanced(ix, nqt) : ix;
+  const int kvh = uni(h / (a.nh / a.nkv));
   const int q0 = qt * kRows + wid * 32;
-  const int klen = a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk;
-  const int start = a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0;
+  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
+  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
   const int pos0 = start + q0;
   const float c = a.scale * kLog2e;
   const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
-  const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
-  const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
-  const float* kbp = BIAS && a.key_bias ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const bool rel = MODE == kRel || (MODE == kKeys && a.table);
 
   Frag<T> qf[2][DS];
 #pragma unroll
@@ -304,116 +425,128 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void fwd_kernel(Args
   const int kend = a.causal ? min(klen, last + 1) : klen;
   const int nt = kend > 0 ? (kend + KT - 1) / KT : 0;
 
-  Tile<T, D, KT> kr, vr;
-  float kbr = 0.f;
+  const Reader<T, D> rd(lane);
+  Tile<T, D, KT> kr((const T*)a.k.p + b * a.k.sb + kvh * a.k.sh, a.k.ss, a.hd, tid);
+  Tile<T, D, KT> vr((const T*)a.v.p + b * a.v.sb + kvh * a.v.sh, a.v.ss, a.hd, tid);
+  float kbr = 0.f, kbn[Tile<T, D, KT>::N];
+  if (MODE == kKeys) row_bias(kbn, kr.row, kbp + grp * KT, klen - grp * KT);
   auto fetch = [&](int t) {
-    kr.load(kp + (long long)t * KT * a.k.ss, a.k.ss, klen - t * KT, a.hd, tid);
-    vr.load(vp + (long long)t * KT * a.v.ss, a.v.ss, klen - t * KT, a.hd, tid);
-    if (BIAS && kbp) {
-      kr.load_bias(kbp + t * KT, klen - t * KT, tid);
-      vr.load_bias(kbp + t * KT, klen - t * KT, tid);
-      if (tid < KT) kbr = t * KT + tid < klen ? to_score_units(a, kbp[t * KT + tid]) : -INFINITY;
-    }
-  };
-  auto put = [&](int buf) {
-    char* kimg = smem + buf * 2 * IMG;
-    if (BIAS && kbp) {
-      kr.store_masked(kimg, tid);
-      vr.store_masked(kimg + IMG, tid);
-      if (tid < KT) kbl[buf * KT + tid] = kbr;
+    char* img = mem + (t / GROUPS & 1) * 2 * IMG;
+    const int left = klen - t * KT;
+    if (MODE == kKeys) {
+      kr.load_masked(t, left, img, wid, kbn);
+      vr.load_masked(t, left, img + IMG, wid, kbn);
+      if (tid < KT) kbr = tid < left ? kbp[t * KT + tid] : -INFINITY;
+      row_bias(kbn, kr.row, kbp + (t + GROUPS) * KT, left - GROUPS * KT);          // (the next tile's loads must not wait for these)
     } else {
-      kr.store(kimg, tid);
-      vr.store(kimg + IMG, tid);
+      kr.load(t, left, img, wid);
+      vr.load(t, left, img + IMG, wid);
     }
   };
-  if (BIAS && a.table) fill_band(a, h, band, tid);
-  if (nt > 0) {
-    fetch(0);
-    put(0);
-  }
+  auto put = [&](int t) {
+    char* img = mem + (t / GROUPS & 1) * 2 * IMG;
+    kr.put(img);
+    vr.put(img + IMG);
+    if (MODE == kKeys && tid < KT) kbl[(t / GROUPS & 1) * KT + tid] = to_score_units(a, kbr);
+    loads_done();
+  };
+  if (grp < nt) fetch(grp);
+  if (rel && grp == 0) fill_band(a, h, band, tid);
+  if (grp < nt) put(grp);
   __syncthreads();
-  for (int t = 0; t < nt; ++t) {
-    const char* kimg = smem + (t & 1) * 2 * IMG;
+  for (int t = grp; t - grp < nt; t += GROUPS) {        // (the groups take turns; all of them keep step)
+    const char* kimg = mem + (t / GROUPS & 1) * 2 * IMG;
     const char* vimg = kimg + IMG;
     const int kt = t * KT;
-    if (t + 1 < nt) fetch(t + 1);
+    if (t + GROUPS < nt) fetch(t + GROUPS);
     // a wave whose rows all end before this tile, or that has no rows, only keeps step
-    if (q0 < a.Sq && (!a.causal || kt <= pos0 + 31)) {
+    if (t < nt && q0 < a.Sq && (!a.causal || kt <= pos0 + 31)) {
       f32x4 s[JB][2];
-      if (BIAS) {
-        const float* kb = kbl + (t & 1) * KT;
 #pragma unroll
-        for (int jb = 0; jb < JB; ++jb) {
-          const f32x4 x = kbp ? *reinterpret_cast<const f32x4*>(kb + jb * 16 + g * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
-          s[jb][0] = x;
-          s[jb][1] = x;
+      for (int jb = 0; jb < JB; ++jb) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (MODE == kKeys) x = *reinterpret_cast<const f32x4*>(kbl + (t / GROUPS & 1) * KT + jb * 16 + g * 4);
+        s[jb][0] = x;
+        s[jb][1] = x;
+      }
+      if (rel) {
+        if (kt + KT - 1 - pos0 <= -a.max_dist || kt - (pos0 + 31) >= a.right) {
+          const float x = kt < pos0 ? band[0] : band[a.max_dist + a.right + 2 * kMargin];
+#pragma unroll
+          for (int jb = 0; jb < JB; ++jb) { s[jb][0] += x; s[jb][1] += x; }
+        } else {
+          const float* at = band + (kt + 4 * g - pos0 - fr + a.max_dist + kMargin);
+          f32x4 x[JB + 1];
+#pragma unroll
+          for (int j = 0; j <= JB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[j][r] = at[(j - 1) * 16 + r];
+#pragma unroll
+          for (int jb = 0; jb < JB; ++jb) { s[jb][0] += x[jb + 1]; s[jb][1] += x[jb]; }
         }
-        if (a.table) {
-          if (kt + KT - 1 - pos0 <= -a.max_dist || kt - (pos0 + 31) >= a.right) {
-            const float x = kt < pos0 ? band[0] : band[a.max_dist + a.right + 2 * kMargin];
-#pragma unroll
-            for (int jb = 0; jb < JB; ++jb) { s[jb][0] += x; s[jb][1] += x; }
-          } else {
-            const float* at = band + (kt + 4 * g - pos0 - fr + a.max_dist + kMargin);
-            f32x4 x[JB + 1];
-#pragma unroll
-            for (int j = 0; j <= JB; ++j)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) x[j][r] = at[(j - 1) * 16 + r];
-#pragma unroll
-            for (int jb = 0; jb < JB; ++jb) { s[jb][0] += x[jb + 1]; s[jb][1] += x[jb]; }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int jb = 0; jb < JB; ++jb) { s[jb][0] = f32x4{0.f, 0.f, 0.f, 0.f}; s[jb][1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
       }
 #pragma unroll
       for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb) {
           Frag<T> kf;
-          frag_row<ST>(kf, kimg, jb * 16, ks, lane);
+          rd.read_row(kf, kimg, jb * 16, ks);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) s[jb][qb] = mma(kf, qf[qb][ks], s[jb][qb]);
         }
       if (kt + KT > klen || (a.causal && kt + KT - 1 > pos0)) {
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-          const int end = a.causal ? min(klen, pos0 + qb * 16 + fr + 1) : klen;
+          const int end = (a.causal ? min(klen, pos0 + qb * 16 + fr + 1) : klen) - kt - 4 * g;
 #pragma unroll
           for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (kt + jb * 16 + 4 * g + r >= end) s[jb][qb][r] = -INFINITY;
+              if (jb * 16 + r >= end) s[jb][qb][r] = -INFINITY;
+        }
+      }
+      // The maximum that is taken off need not be the row's exact one, only near enough for the exponentials: it moves,
+      // and O and the sums with it, when a row outgrows it by a factor of 2^8, which after the first tiles hardly happens.
+      // scale > 0: the maximum commutes with the scaling. With key biases the difference is taken in score units, where
+      // it is exact: the product of a lowest-value mask with c is rounded by far more than 1.
+      float mx[2];
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        mx[qb] = -INFINITY;
+#pragma unroll
+        for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx[qb] = fmaxf(mx[qb], s[jb][qb][r]);
+        mx[qb] = group_max(mx[qb]);
+        if (MODE != kKeys) mx[qb] *= c;
+      }
+      const float lim = MODE == kKeys ? 8.f / c : 8.f;
+      const bool grow0 = mx[0] > m[0] + lim, grow1 = mx[1] > m[1] + lim;
+      if (__any(grow0 || grow1)) {
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          const float mn = (qb ? grow1 : grow0) ? mx[qb] : m[qb];
+          const float alpha = mn == m[qb] ? 1.f : fexp2(MODE == kKeys ? (m[qb] - mn) * c : m[qb] - mn);
+          m[qb] = mn;
+          l[qb] *= alpha;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
         }
       }
       Frag<T> pf[2][KT / 32];
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[jb][qb][r]);
-        // scale > 0: the maximum commutes with the scaling. With biases the difference is taken in score units, where it
-        // is exact: the product of a lowest-value mask with c is rounded by far more than 1
-        const float mn = fmaxf(m[qb], BIAS ? group_max(mx) : group_max(mx) * c);
-        const float ref = mn == -INFINITY ? 0.f : mn;                // nothing seen yet: every term below is exp2(-inf)
-        const float alpha = fexp2(BIAS ? (m[qb] - ref) * c : m[qb] - ref);
-        m[qb] = mn;
+        const float ref = m[qb] == -INFINITY ? 0.f : m[qb];          // nothing seen yet: every term is exp2(-inf)
         float sum = 0.f;
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = fexp2(BIAS ? (s[jb][qb][r] - ref) * c : fmaf(s[jb][qb][r], c, -ref));
+            const float p = fexp2(MODE == kKeys ? (s[jb][qb][r] - ref) * c : fmaf(s[jb][qb][r], c, -ref));
             s[jb][qb][r] = p;
             sum += p;
           }
-        l[qb] = l[qb] * alpha + sum;                                 // per lane; combined over the lane group at the end
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
+        l[qb] += sum;                                                // per lane; combined over the lane group at the end
 #pragma unroll
         for (int ks = 0; ks < KT / 32; ++ks) pack(pf[qb][ks], s[2 * ks][qb], s[2 * ks + 1][qb]);
       }
@@ -422,18 +555,43 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void fwd_kernel(Args
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           Frag<T> vf;
-          frag_tr<ST>(vf, vimg, db * 16, ks, lane);
+          rd.read_tr(vf, vimg, db, ks);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) o[db][qb] = mma(vf, pf[qb][ks], o[db][qb]);
         }
     }
-    if (t + 1 < nt) put((t + 1) & 1);
+    if (t + GROUPS < nt) put(t + GROUPS);
     __syncthreads();
+  }
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) l[qb] = group_sum(l[qb]);
+  if (GROUPS > 1) {                                     // join: the second group's sums through its images' memory
+    float* oj = reinterpret_cast<float*>(smem + 4 * IMG + 8 * KT) + wid * 32 * D, *mj = band + (wid * 2) * 64;
+    if (grp == 1) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(oj + ((qb * DB + db) * 64 + lane) * 4) = o[db][qb];
+        mj[qb * 64 + lane] = m[qb];
+        mj[4 * 2 * 64 + qb * 64 + lane] = l[qb];
+      }
+    }
+    __syncthreads();
+    if (grp == 1) return;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const float m1 = mj[qb * 64 + lane], l1 = mj[4 * 2 * 64 + qb * 64 + lane], mm = fmaxf(m[qb], m1), ref = mm == -INFINITY ? 0.f : mm;
+      const float f0 = fexp2(MODE == kKeys ? (m[qb] - ref) * c : m[qb] - ref), f1 = fexp2(MODE == kKeys ? (m1 - ref) * c : m1 - ref);
+      m[qb] = mm;
+      l[qb] = l[qb] * f0 + l1 * f1;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db][qb] = o[db][qb] * f0 + *reinterpret_cast<const f32x4*>(oj + ((qb * DB + db) * 64 + lane) * 4) * f1;
+    }
   }
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const int q = q0 + qb * 16 + fr;
-    const float lt = group_sum(l[qb]);
+    const float lt = l[qb];
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
     if (q < a.Sq) {
       T* row = (T*)a.out.p + b * a.out.sb + (long long)q * a.out.ss + h * a.out.sh;
@@ -459,7 +617,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void fwd_kernel(Args
 constexpr int kFewRows = 32, kFewKeys = 32;
 
 // O and the row's statistics of row r of a key head's rows
-template <typename T, bool BIAS>
+template <typename T, int MODE>
 __device__ __forceinline__ void few_store(const Args& a, int b, int kvh, int group, int r, int d, float mm, float lt,
                                           const f32x4& acc, float c) {
   const int i = r / group, h = kvh * group + r - i * group;
@@ -467,14 +625,14 @@ __device__ __forceinline__ void few_store(const Args& a, int b, int kvh, int gro
   if (d < a.hd) store4((T*)a.out.p + b * a.out.sb + (long long)i * a.out.ss + h * a.out.sh + d, acc * inv);
   if (d == 0 && a.stat) {
     const long long at = ((long long)b * a.nh + h) * a.Sq + i, n = (long long)a.B * a.nh * a.Sq;
-    a.stat[at] = lt == 0.f ? INFINITY : (BIAS ? mm : mm * c);        // the units of fwd_kernel
+    a.stat[at] = lt == 0.f ? INFINITY : (MODE == kKeys ? mm : mm * c);        // the units of fwd_kernel
     a.stat[n + at] = lt == 0.f ? 0.f : flog2(lt);
   }
 }
 
-template <typename T, int D, int QB, bool BIAS>
+template <typename T, int D, int QB, int MODE>
 __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
-  constexpr int DB = D / 16, DS = D / 32, ST = row_stride<T, D>(), IMG = kFewKeys * ST, JOIN = QB * 16 * (D + 4) * 4;
+  constexpr int DB = D / 16, DS = D / 32, IMG = kFewKeys * row_stride<T, D>(), JOIN = QB * 16 * (D + 4) * 4;
   constexpr int kChunk = 16 / (int)sizeof(T), kPerRow = D / kChunk, NV = kFewKeys * kPerRow / 64;
   extern __shared__ __attribute__((aligned(16))) char smem[];      // [4 waves][V image, then O], [4][2][rows], table
   constexpr int REGION = IMG > JOIN ? IMG : JOIN;
@@ -483,19 +641,20 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
   char* vimg = smem + wid * REGION;
   float* ml = reinterpret_cast<float*>(smem + 4 * REGION);
   float* tab = ml + 4 * 2 * QB * 16;
-  const int group = a.nh / a.nkv, rows = a.Sq * group;
-  const int split = blockIdx.x % a.splits, bk = blockIdx.x / a.splits, b = bk / a.nkv, kvh = bk - b * a.nkv;
-  const int klen = a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk;
-  const int start = a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0;
+  const int group = uni(a.nh / a.nkv), rows = a.Sq * group;
+  const int bk = uni(blockIdx.x / a.splits), split = blockIdx.x - bk * a.splits, b = uni(bk / a.nkv), kvh = bk - b * a.nkv;
+  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
+  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
   const float c = a.scale * kLog2e;
   const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
-  const float* kbp = BIAS && a.key_bias ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const bool rel = MODE == kRel || (MODE == kKeys && a.table);
 
-  if (BIAS && a.table) {
+  if (rel) {
     for (int i = tid; i < group * a.buckets; i += 256) {
       const int hg = i / a.buckets;
-      tab[i] = to_score_units(a, table_at(a, i - hg * a.buckets, kvh * group + hg));
+      tab[i] = learned_bias(a, table_at(a, i - hg * a.buckets, kvh * group + hg));
     }
     __syncthreads();
   }
@@ -524,23 +683,20 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
   const int nt = kend > 0 ? (kend + kFewKeys - 1) / kFewKeys : 0, per = (nt + a.splits - 1) / a.splits;
   const int t1 = min(nt, (split + 1) * per);
 
+  const Reader<T, D> rd(lane);
   Frag<T> kf[2][DS];
   u32x4_t vr[NV];
-  float kbv[NV];
   f32x4 kb[2];
   const unsigned kld = (unsigned)a.k.ss * (unsigned)sizeof(T), vld = (unsigned)a.v.ss * (unsigned)sizeof(T);
-  auto rsrc = [&](const T* base, unsigned ld, int left) {
-    left = min(left, kFewKeys);
-    const unsigned bytes = (unsigned)(left - 1) * ld + (unsigned)a.hd * (unsigned)sizeof(T);
-    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
-  };
   auto fetch = [&](int t) {                              // (left >= 1: the tile starts before kend)
     const int k0 = t * kFewKeys, left = klen - k0;
-    const __amdgpu_buffer_rsrc_t kr = rsrc(kp + (long long)k0 * a.k.ss, kld, left), vs = rsrc(vp + (long long)k0 * a.v.ss, vld, left);
+    const unsigned used = (unsigned)a.hd * (unsigned)sizeof(T);
+    const __amdgpu_buffer_rsrc_t kr = tile_rsrc(kp + (long long)k0 * a.k.ss, kld, used, left, kFewKeys);
+    const __amdgpu_buffer_rsrc_t vs = tile_rsrc(vp + (long long)k0 * a.v.ss, vld, used, left, kFewKeys);
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb) {
       const int row = jb * 16 + fr;
-      const bool in = row < left && !(BIAS && kbp && kbp[k0 + row] == -INFINITY);
+      const bool in = row < left && !(MODE == kKeys && kbp[k0 + row] == -INFINITY);
 #pragma unroll
       for (int ks = 0; ks < DS; ++ks) {
         const int e = ks * 32 + g * 8;
@@ -551,7 +707,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
           w[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(off == 0xffffffffu ? off : off + 16u * i), 0, 0));
         __builtin_memcpy(&kf[jb][ks], w, sizeof(Frag<T>));
       }
-      if (BIAS && kbp) {
+      if (MODE == kKeys) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int k = k0 + jb * 16 + 4 * g + r;
@@ -562,7 +718,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int p = u * 64 + lane, row = p / kPerRow, ch = p - row * kPerRow;
-      const bool in = row < left && ch * kChunk < a.hd && !(BIAS && kbp && kbp[k0 + row] == -INFINITY);
+      const bool in = row < left && ch * kChunk < a.hd && !(MODE == kKeys && kbp[k0 + row] == -INFINITY);
       vr[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vs, (int)(in ? (unsigned)row * vld + (unsigned)ch * 16u : 0xffffffffu), 0, 0));
     }
   };
@@ -577,8 +733,8 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         s[jb][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (BIAS && kbp) s[jb][qb] = kb[jb];
-        if (BIAS && a.table) {
+        if (MODE == kKeys) s[jb][qb] = kb[jb];
+        if (rel) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[jb][qb][r] += tb[qb][bucket_of(a, kt + jb * 16 + 4 * g + r - pos[qb])];
         }
@@ -593,7 +749,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int p = u * 64 + lane, row = p / kPerRow, ch = p - row * kPerRow;
-      *reinterpret_cast<u32x4_t*>(vimg + row * ST + ch * 16) = vr[u];
+      *reinterpret_cast<u32x4_t*>(vimg + chunk_at<T, D>(row, ch)) = vr[u];
     }
     if (t + 4 < t1) fetch(t + 4);
     Frag<T> pf[QB];
@@ -628,7 +784,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
       Frag<T> vf;
-      frag_tr<ST>(vf, vimg, db * 16, 0, lane);
+      rd.read_tr(vf, vimg, db, 0);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) o[db][qb] = mma(vf, pf[qb], o[db][qb]);
     }
@@ -669,14 +825,14 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
       float* st = a.part + (long long)a.splits * n_rows * D + (long long)split * 2 * n_rows;
       if (d == 0) { st[row] = mm; st[n_rows + row] = lt; }
     } else {
-      few_store<T, BIAS>(a, b, kvh, group, r, d, mm, lt, acc, c);
+      few_store<T, MODE>(a, b, kvh, group, r, d, mm, lt, acc, c);
     }
   }
 }
 
 // One workgroup a row: its threads share out the row's splits as well as its elements, so that no thread waits for more
 // than a few loads one after the other (one wave a row, walking the splits: 13.5 us where few_kernel itself takes 12).
-template <typename T, int D, bool BIAS>
+template <typename T, int D, int MODE>
 __global__ __launch_bounds__(256) void few_join_kernel(Args a) {
   constexpr int L = D / 4, S = 256 / L;                  // lanes of a row, splits taken at a time
   __shared__ __attribute__((aligned(16))) float red[S][D + 4];
@@ -705,7 +861,7 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a) {
   if (sub == 0) {
     for (int s = 1; s < S && s < a.splits; ++s) acc += *reinterpret_cast<const f32x4*>(&red[s][d]);
     const int bk = (int)(row / rows), b = bk / a.nkv;
-    few_store<T, BIAS>(a, b, bk - b * a.nkv, group, (int)(row - (long long)bk * rows), d, stats[0], stats[1], acc, c);
+    few_store<T, MODE>(a, b, bk - b * a.nkv, group, (int)(row - (long long)bk * rows), d, stats[0], stats[1], acc, c);
   }
 }
 
@@ -716,8 +872,8 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a) {
 // the lanes of one distance together, and a lane that wraps around carries a value of distance 16 J + 16 - ..., which is
 // exactly the place of the NEXT block's rotation: selecting between e_J and e_(J-1) before the rotation makes every lane
 // right. Three such rotations fold r away, then one by 4 g per lane group folds g, and two half swaps sum the lane groups
-// and put four blocks side by side: 64 lanes with 64 consecutive distances, one LDS addition per tile where one per
-// register with colliding lanes (ds_add_f32, 20 a tile) took three quarters of the kernel (0.54 ms instead of 0.16 at
+// and put two blocks side by side: 32 lanes with 32 consecutive distances, one LDS addition per 32 x 32 scores where one
+// per register with colliding lanes (ds_add_f32, 12 of them) took three quarters of the kernel (0.54 ms instead of 0.16 at
 // 64 x 512 tokens, 12 heads of 64). Every sum has a fixed order.
 struct DiagonalSums {
   f32x4 carry, prev;                 // block not complete yet (its other query block comes with the next tile), block J - 1
@@ -742,13 +898,12 @@ struct DiagonalSums {
     const unsigned x = r[0], y = r[1];
     return __uint_as_float(x) + __uint_as_float(y);
   }
-  // gx[j]: block diagonal j - 1 of the tile, j = 0 .. JB. Completes blocks -1 .. JB - 2; the sum of distance
-  // 16 (b - 1) - fr (relative to key 0 of the tile and query 0 of the wave) is returned in lane group b.
-  template <int JB>
-  __device__ __forceinline__ float add(const f32x4 (&gx)[JB + 1], int fr, int g) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+  // gx[j]: block diagonal j - 1 of 32 keys x 32 queries, j = 0, 1, 2. Completes blocks -1 and 0: the sum of distance
+  // 16 (b - 1) - fr (relative to the first key and query) is returned in lane group b = 0, 1.
+  __device__ __forceinline__ float add(const f32x4 (&gx)[3], int fr, int g) {
+    float v[2];
 #pragma unroll
-    for (int b = 0; b < JB; ++b) {
+    for (int b = 0; b < 2; ++b) {
       const f32x4 e = b == 0 ? gx[0] + carry : gx[b];
       float t = e[0];
       t += rot<1>(fr < 1 ? prev[1] : e[1]);
@@ -761,40 +916,43 @@ struct DiagonalSums {
       x = __builtin_amdgcn_update_dpp(x, x, 0x120 + 8, 0xc, 0xf, false);       // 2 and 3: by 8
       v[b] = __int_as_float(x);
     }
-    carry = gx[JB];
-    return rows(halves(v[0], v[2]), halves(v[1], v[3]));
+    carry = gx[2];
+    const float r = rows(v[0], v[1]);                    // lane groups 0, 2: block 0 of groups (0, 1), (2, 3); 1, 3: block 1
+    return halves(r, r);
   }
 };
 
 // A workgroup owns 128 query rows and walks the keys. It also writes D = rowsum(dO * O) for the dK / dV kernel and sums
-// the relative bias's gradient: by distance (DiagonalSums, into a band of the wave's own) where a tile touches the band,
+// the relative bias's gradient: by distance (DiagonalSums, into a band of the wave's own, where no two lanes of an
+// addition meet) where a tile touches the band,
 // into one of two registers where it lies beyond.
-template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_dq_kernel(Args a) {
-  constexpr int KT = key_tile<T>(), JB = KT / 16, DB = D / 16, DS = D / 32, ST = row_stride<T, D>(), IMG = KT * ST;
+template <typename T, int D, int MODE, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <= 64 && MODE == kPlain && GROUPS == 1 ? 3 : 2) : GROUPS)) void bwd_dq_kernel(Args a) {
+  constexpr int KT = key_tile<T>(), DB = D / 16, DS = D / 32, IMG = Tile<T, D, KT>::IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V], [2][key bias], band, band gradients
-  float* kbl = reinterpret_cast<float*>(smem + 4 * IMG);
-  float* band = kbl + 2 * KT;
-  const int nband = BIAS && a.table ? band_size(a) : 0;
-  float* gband = band + nband;                                     // [4 waves][nband], then 8 far sums
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x & 255, lane = tid & 63, wid = uni(tid >> 6), grp = GROUPS > 1 ? uni(threadIdx.x >> 8) : 0;
+  char* mem = smem + grp * (4 * IMG + 8 * KT);                     // the group's tile images and key biases
+  float* kbl = reinterpret_cast<float*>(mem + 4 * IMG);
+  float* band = reinterpret_cast<float*>(smem + GROUPS * (4 * IMG + 8 * KT));
+  const bool rel = MODE == kRel || (MODE == kKeys && a.table);
+  const int nband = rel ? band_size(a) : 0;
+  float* gband = band + nband;                                     // [waves][nband], then two far sums a wave
   const int fr = lane & 15, g = lane >> 4;
   const int nqt = (a.Sq + kRows - 1) / kRows;
-  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int qt = a.causal ? nqt - 1 - id % nqt : id % nqt, bh = id / nqt, b = bh / a.nh, h = bh - b * a.nh;
-  const int kvh = h / (a.nh / a.nkv);
+  const int id = uni(xcd_contiguous(blockIdx.x, gridDim.x));
+  const int bh = uni(id / nqt), ix = id - bh * nqt, b = uni(bh / a.nh), h = bh - b * a.nh;
+  const int qt = a.causal ? nqt - 1 - balanced(ix, nqt) : ix;
+  const int kvh = uni(h / (a.nh / a.nkv));
   const int q0 = qt * kRows + wid * 32;
-  const int klen = a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk;
-  const int start = a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0;
+  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
+  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
   const int pos0 = start + q0;
   const float c = a.scale * kLog2e;
   const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
-  const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
-  const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
   const T* op = (const T*)a.out.p + b * a.out.sb + h * a.out.sh;
   const T* dop = (const T*)a.dout.p + b * a.dout.sb + h * a.dout.sh;
-  const float* kbp = BIAS && a.key_bias ? a.key_bias + (long long)b * a.Sk : nullptr;
-  const bool want_tab = BIAS && a.dtab;
+  const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const bool want_tab = rel && a.dtab;
 
   Frag<T> qf[2][DS], dof[2][DS];
   float m2[2], ll[2], dl[2];
@@ -813,10 +971,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
     }
     const long long i = ((long long)b * a.nh + h) * a.Sq + qc, n = (long long)a.B * a.nh * a.Sq;
     dl[qb] = group_sum(part);
-    if (g == 0 && q < a.Sq) a.delta[i] = dl[qb];
     m2[qb] = q < a.Sq ? a.stat[i] : INFINITY;            // rows past the end: probabilities 0
     ll[qb] = q < a.Sq ? a.stat[n + i] : 0.f;
-    if (!BIAS) m2[qb] += ll[qb];
+    if (MODE != kKeys) m2[qb] += ll[qb];
+    if (g == 0 && grp == 0) {
+      float* w = a.rows + row_tile(a, bh, q >> 6) + (q & 63);
+      w[0] = m2[qb];
+      w[64] = ll[qb];
+      w[128] = -dl[qb];
+    }
   }
   f32x4 dq[DB][2];
 #pragma unroll
@@ -829,82 +992,77 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
   const int kend = a.causal ? min(klen, last + 1) : klen;
   const int nt = kend > 0 ? (kend + KT - 1) / KT : 0;
 
-  Tile<T, D, KT> kr, vr;
-  float kbr = 0.f;
+  const Reader<T, D> rd(lane);
+  Tile<T, D, KT> kr((const T*)a.k.p + b * a.k.sb + kvh * a.k.sh, a.k.ss, a.hd, tid);
+  Tile<T, D, KT> vr((const T*)a.v.p + b * a.v.sb + kvh * a.v.sh, a.v.ss, a.hd, tid);
+  float kbr = 0.f, kbn[Tile<T, D, KT>::N];
+  if (MODE == kKeys) row_bias(kbn, kr.row, kbp + grp * KT, klen - grp * KT);
   auto fetch = [&](int t) {
-    kr.load(kp + (long long)t * KT * a.k.ss, a.k.ss, klen - t * KT, a.hd, tid);
-    vr.load(vp + (long long)t * KT * a.v.ss, a.v.ss, klen - t * KT, a.hd, tid);
-    if (BIAS && kbp) {
-      kr.load_bias(kbp + t * KT, klen - t * KT, tid);
-      vr.load_bias(kbp + t * KT, klen - t * KT, tid);
-      if (tid < KT) kbr = t * KT + tid < klen ? to_score_units(a, kbp[t * KT + tid]) : -INFINITY;
-    }
-  };
-  auto put = [&](int buf) {
-    char* kimg = smem + buf * 2 * IMG;
-    if (BIAS && kbp) {
-      kr.store_masked(kimg, tid);
-      vr.store_masked(kimg + IMG, tid);
-      if (tid < KT) kbl[buf * KT + tid] = kbr;
+    char* img = mem + (t / GROUPS & 1) * 2 * IMG;
+    const int left = klen - t * KT;
+    if (MODE == kKeys) {
+      kr.load_masked(t, left, img, wid, kbn);
+      vr.load_masked(t, left, img + IMG, wid, kbn);
+      if (tid < KT) kbr = tid < left ? kbp[t * KT + tid] : -INFINITY;
+      row_bias(kbn, kr.row, kbp + (t + GROUPS) * KT, left - GROUPS * KT);          // (the next tile's loads must not wait for these)
     } else {
-      kr.store(kimg, tid);
-      vr.store(kimg + IMG, tid);
+      kr.load(t, left, img, wid);
+      vr.load(t, left, img + IMG, wid);
     }
   };
-  if (BIAS && a.table) fill_band(a, h, band, tid);
+  auto put = [&](int t) {
+    char* img = mem + (t / GROUPS & 1) * 2 * IMG;
+    kr.put(img);
+    vr.put(img + IMG);
+    if (MODE == kKeys && tid < KT) kbl[(t / GROUPS & 1) * KT + tid] = to_score_units(a, kbr);
+    loads_done();
+  };
+  if (grp < nt) fetch(grp);
+  if (rel && grp == 0) fill_band(a, h, band, tid);
   if (want_tab)
-    for (int i = tid; i < 4 * nband; i += 256) gband[i] = 0.f;
-  float* gmine = gband + wid * nband;
+    for (int i = threadIdx.x; i < 4 * GROUPS * nband; i += 256 * GROUPS) gband[i] = 0.f;
+  float* gmine = gband + (grp * 4 + wid) * nband;
   DiagonalSums diag;
   diag.reset();
   int diag_at = 0;                                       // band entry of the next tile's first distance; 0: no tile yet
-  if (nt > 0) {
-    fetch(0);
-    put(0);
-  }
+  auto finish_diagonals = [&]() {                        // what the last block on the band left incomplete
+    const f32x4 none[3] = {};
+    const float v = diag.add(none, fr, g);
+    if (g < 2) atomicAdd(gmine + diag_at + 16 * (g - 1) - fr, v);
+    diag.reset();
+    diag_at = 0;
+  };
+  if (grp < nt) put(grp);
   __syncthreads();
-  for (int t = 0; t < nt; ++t) {
-    const char* kimg = smem + (t & 1) * 2 * IMG;
+  for (int t = grp; t - grp < nt; t += GROUPS) {        // (the groups take turns; all of them keep step)
+    const char* kimg = mem + (t / GROUPS & 1) * 2 * IMG;
     const char* vimg = kimg + IMG;
     const int kt = t * KT;
-    if (t + 1 < nt) fetch(t + 1);
-    if (q0 < a.Sq && (!a.causal || kt <= pos0 + 31)) {
-      const bool far = BIAS && a.table && (kt + KT - 1 - pos0 <= -a.max_dist || kt - (pos0 + 31) >= a.right);
+    if (t + GROUPS < nt) fetch(t + GROUPS);
+    if (t < nt && q0 < a.Sq && (!a.causal || kt <= pos0 + 31)) {
+      const bool far = rel && (kt + KT - 1 - pos0 <= -a.max_dist || kt - (pos0 + 31) >= a.right);
       const int at0 = kt + 4 * g - pos0 - fr + a.max_dist + kMargin;    // band entry of (key 4 g of block 0, query fr)
-      f32x4 x[JB + 1];
-      if (BIAS && a.table) {
-        if (far) {
-          const float v = kt < pos0 ? band[0] : band[nband - 1];
-#pragma unroll
-          for (int j = 0; j <= JB; ++j) x[j] = f32x4{v, v, v, v};
-        } else {
-#pragma unroll
-          for (int j = 0; j <= JB; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[j][r] = band[at0 + (j - 1) * 16 + r];
-        }
-      } else if (BIAS) {
-#pragma unroll
-        for (int j = 0; j <= JB; ++j) x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-      f32x4 gx[JB + 1];
-      if (BIAS) {
-#pragma unroll
-        for (int j = 0; j <= JB; ++j) gx[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+      const float xf = rel && far ? (kt < pos0 ? band[0] : band[nband - 1]) : 0.f;
       const bool edge = kt + KT > klen || (a.causal && kt + KT - 1 > pos0);
 #pragma unroll
       for (int hf = 0; hf < KT / 32; ++hf) {
-        f32x4 s[2][2], dp[2][2];
+        f32x4 s[2][2], dp[2][2], x[3];                   // x: key block minus query block of the half -1, 0, 1
+#pragma unroll
+        for (int j = 0; j < 3; ++j) x[j] = f32x4{xf, xf, xf, xf};
+        if (rel && !far) {
+#pragma unroll
+          for (int j = 0; j < 3; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[j][r] = band[at0 + (hf * 2 + j - 1) * 16 + r];
+        }
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
-          const int jb = hf * 2 + jj;
           f32x4 kb = {0.f, 0.f, 0.f, 0.f};
-          if (BIAS && kbp) kb = *reinterpret_cast<const f32x4*>(kbl + (t & 1) * KT + jb * 16 + g * 4);
+          if (MODE == kKeys) kb = *reinterpret_cast<const f32x4*>(kbl + (t / GROUPS & 1) * KT + (hf * 2 + jj) * 16 + g * 4);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) {
-            s[jj][qb] = BIAS ? kb + x[jb + 1 - qb] : f32x4{0.f, 0.f, 0.f, 0.f};
-            dp[jj][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+            s[jj][qb] = MODE == kKeys ? kb + x[jj + 1 - qb] : MODE == kRel ? x[jj + 1 - qb] : f32x4{0.f, 0.f, 0.f, 0.f};
+            dp[jj][qb] = f32x4{-dl[qb], -dl[qb], -dl[qb], -dl[qb]};   // dP - D comes out of the product
           }
         }
 #pragma unroll
@@ -912,8 +1070,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
 #pragma unroll
           for (int jj = 0; jj < 2; ++jj) {
             Frag<T> kf, vf;
-            frag_row<ST>(kf, kimg, (hf * 2 + jj) * 16, ks, lane);
-            frag_row<ST>(vf, vimg, (hf * 2 + jj) * 16, ks, lane);
+            rd.read_row(kf, kimg, (hf * 2 + jj) * 16, ks);
+            rd.read_row(vf, vimg, (hf * 2 + jj) * 16, ks);
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
               s[jj][qb] = mma(kf, qf[qb][ks], s[jj][qb]);
@@ -923,60 +1081,80 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
         if (edge) {
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) {
-            const int end = a.causal ? min(klen, pos0 + qb * 16 + fr + 1) : klen;
+            const int end = (a.causal ? min(klen, pos0 + qb * 16 + fr + 1) : klen) - kt - 4 * g;
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
               for (int r = 0; r < 4; ++r)
-                if (kt + (hf * 2 + jj) * 16 + 4 * g + r >= end) s[jj][qb][r] = -INFINITY;
+                if ((hf * 2 + jj) * 16 + r >= end) s[jj][qb][r] = -INFINITY;
           }
         }
         Frag<T> dsf[2];
+        f32x4 gx[3];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) gx[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
 #pragma unroll
           for (int jj = 0; jj < 2; ++jj) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              // with biases the row maximum may be so large (a row of lowest-value masks) that the logarithm of the
+              // with key biases the row maximum may be so large (a row of lowest-value masks) that the logarithm of the
               // sum is lost next to it: the two are taken off one after the other
-              const float p = fexp2(BIAS ? fmaf(s[jj][qb][r] - m2[qb], c, -ll[qb]) : fmaf(s[jj][qb][r], c, -m2[qb]));
-              s[jj][qb][r] = p * (dp[jj][qb][r] - dl[qb]);
+              const float p = fexp2(MODE == kKeys ? fmaf(s[jj][qb][r] - m2[qb], c, -ll[qb]) : fmaf(s[jj][qb][r], c, -m2[qb]));
+              s[jj][qb][r] = p * dp[jj][qb][r];
             }
-            if (BIAS) gx[hf * 2 + jj + 1 - qb] += s[jj][qb];
+            if (MODE != kPlain) gx[jj + 1 - qb] += s[jj][qb];
           }
           pack(dsf[qb], s[0][qb], s[1][qb]);
+        }
+        if (want_tab) {
+          if (far) {
+            const f32x4 v = gx[0] + gx[1] + gx[2];
+            if (kt < pos0) far_l += (v[0] + v[1]) + (v[2] + v[3]);
+            else far_r += (v[0] + v[1]) + (v[2] + v[3]);
+          } else {
+            // blocks of 32 keys that follow one another hand on what is incomplete; the groups' tiles do not
+            const float v = diag.add(gx, fr, g);
+            diag_at = kt - pos0 + hf * 32 + a.max_dist + kMargin;
+            if (g < 2) atomicAdd(gmine + diag_at + 16 * (g - 1) - fr, v);
+            diag_at += 32;
+            if (GROUPS > 1 && hf == KT / 32 - 1) finish_diagonals();
+          }
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           Frag<T> ktr;
-          frag_tr<ST>(ktr, kimg, db * 16, hf, lane);
+          rd.read_tr(ktr, kimg, db, hf);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) dq[db][qb] = mma(ktr, dsf[qb], dq[db][qb]);
         }
-      }
-      if (want_tab) {
-        if (far) {
-          float v = 0.f;
-#pragma unroll
-          for (int j = 0; j <= JB; ++j) v += (gx[j][0] + gx[j][1]) + (gx[j][2] + gx[j][3]);
-          if (kt < pos0) far_l += v; else far_r += v;
-        } else {                                         // (the tiles on the band follow one another)
-          const float v = diag.template add<JB>(gx, fr, g);
-          diag_at = kt - pos0 + a.max_dist + kMargin;
-          const int i = diag_at + 16 * (g - 1) - fr;
-          if (g < JB && i >= 0) gmine[i] += v;
-          diag_at += KT;
-        }
+        if (D > 64) __builtin_amdgcn_sched_barrier(0);   // the halves interleaved would not fit the registers
       }
     }
-    if (t + 1 < nt) put((t + 1) & 1);
+    if (t + GROUPS < nt) put(t + GROUPS);
     __syncthreads();
+  }
+  if (GROUPS > 1) {                                     // join: the second group's sums through its images' memory
+    float* oj = reinterpret_cast<float*>(smem + 4 * IMG + 8 * KT) + wid * 32 * D;
+    if (grp == 1) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(oj + ((qb * DB + db) * 64 + lane) * 4) = dq[db][qb];
+    }
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dq[db][qb] += *reinterpret_cast<const f32x4*>(oj + ((qb * DB + db) * 64 + lane) * 4);
+    }
   }
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    const int q = q0 + qb * 16 + fr;
-    if (q < a.Sq) {
+    const int q = opaque(q0 + qb * 16 + fr);             // (the rows' addresses are not for the loop to keep)
+    if (q < a.Sq && grp == 0) {
       T* row = (T*)a.dq.p + b * a.dq.sb + (long long)q * a.dq.ss + h * a.dq.sh;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -984,29 +1162,28 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
     }
   }
   if (want_tab) {
-    if (diag_at) {                                       // what the last tile on the band left incomplete
-      f32x4 none[JB + 1];
-#pragma unroll
-      for (int j = 0; j <= JB; ++j) none[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const float v = diag.template add<JB>(none, fr, g);
-      const int i = diag_at + 16 * (g - 1) - fr;
-      if (g < JB && i < nband) gmine[i] += v;
-    }
-    float* fars = gband + 4 * nband;
+    if (diag_at) finish_diagonals();
+    float* fars = gband + 4 * GROUPS * nband;
     far_l = wave_sum(far_l);
     far_r = wave_sum(far_r);
-    if (lane == 0) { fars[wid * 2] = far_l; fars[wid * 2 + 1] = far_r; }
+    if (lane == 0) { fars[(grp * 4 + wid) * 2] = far_l; fars[(grp * 4 + wid) * 2 + 1] = far_r; }
     __syncthreads();
-    for (int i = tid; i < nband; i += 256)               // (no wave reads the band any more)
-      band[i] = (gband[i] + gband[nband + i]) + (gband[2 * nband + i] + gband[3 * nband + i]);
+    for (int i = threadIdx.x; i < nband; i += 256 * GROUPS) {        // (no wave reads the band any more)
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4 * GROUPS; ++w) v += gband[w * nband + i];
+      band[i] = v;
+    }
     __syncthreads();
-    if (tid < a.buckets) {
+    if (threadIdx.x < a.buckets) {
       int lo, hi;
       bucket_range(a, tid, lo, hi);
       float v = 0.f;
       for (int i = lo; i <= hi; ++i) v += band[i + a.max_dist + kMargin];
-      if (lo == -a.max_dist - kMargin && lo <= hi) v += (fars[0] + fars[2]) + (fars[4] + fars[6]);
-      if (hi == a.right + kMargin && lo <= hi) v += (fars[1] + fars[3]) + (fars[5] + fars[7]);
+      if (lo == -a.max_dist - kMargin && lo <= hi)
+        for (int w = 0; w < 4 * GROUPS; ++w) v += fars[w * 2];
+      if (hi == a.right + kMargin && lo <= hi)
+        for (int w = 0; w < 4 * GROUPS; ++w) v += fars[w * 2 + 1];
       a.dtab[(((long long)b * nqt + qt) * a.nh + h) * a.buckets + tid] = v;
     }
   }
@@ -1015,31 +1192,35 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
 // ================================================================================================== backward: dK, dV
 // A workgroup owns 128 keys of one key head, a wave 32 of them, and walks the query tiles of every query head of the
 // group: gradients of shared heads are summed in the accumulators. The KEY rides on the lane here.
-template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_dkdv_kernel(Args a) {
-  constexpr int QT = key_tile<T>(), IB = QT / 16, DB = D / 16, DS = D / 32, ST = row_stride<T, D>(), IMG = QT * ST;
-  extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q | dO], [2][maximum | log sum | D], band
-  float* stl = reinterpret_cast<float*>(smem + 4 * IMG);
-  float* band = stl + 2 * 3 * QT;
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+template <typename T, int D, int MODE, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <= 64 && MODE == kPlain && GROUPS == 1 ? 3 : 2) : GROUPS)) void bwd_dkdv_kernel(Args a) {
+  constexpr int QT = key_tile<T>(), DB = D / 16, DS = D / 32, IMG = Tile<T, D, QT>::IMG;
+  extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][Q | dO], [2][row statistics], band
+  const int tid = threadIdx.x & 255, lane = tid & 63, wid = uni(tid >> 6), grp = GROUPS > 1 ? uni(threadIdx.x >> 8) : 0;
+  char* mem = smem + grp * (4 * IMG + 8 * kRowStats);              // the group's tile images and row statistics
+  float* stl = reinterpret_cast<float*>(mem + 4 * IMG);
+  float* band = reinterpret_cast<float*>(smem + GROUPS * (4 * IMG + 8 * kRowStats));
   const int fr = lane & 15, g = lane >> 4;
-  const int nkt = (a.Sk + kRows - 1) / kRows, group = a.nh / a.nkv;
-  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bk = id / nkt, b = bk / a.nkv, kvh = bk - b * a.nkv;
-  const int kb0 = (id - bk * nkt) * kRows, k0 = kb0 + wid * 32;
-  const int klen = a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk;
-  const int start = a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0;
+  const int nkt = (a.Sk + kRows - 1) / kRows, group = uni(a.nh / a.nkv);
+  const int id = uni(xcd_contiguous(blockIdx.x, gridDim.x));
+  const int per = nkt * a.ksplits, bk = uni(id / per), b = uni(bk / a.nkv), kvh = bk - b * a.nkv;
+  const int split = uni((id - bk * per) / nkt), ix = id - bk * per - split * nkt, heads = uni(group / a.ksplits);
+  const int kb0 = (a.causal ? balanced(ix, nkt) : ix) * kRows, k0 = kb0 + wid * 32;
+  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
+  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
   const float c = a.scale * kLog2e;
   const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
-  const float* kbp = BIAS && a.key_bias ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
+  const bool rel = MODE == kRel || (MODE == kKeys && a.table);
+  const Reader<T, D, (D <= 64)> rd(lane);
 
   Frag<T> kf[2][DS], vf[2][DS];
   float kbias[2];
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
     const int k = k0 + kb * 16 + fr, kc = min(k, a.Sk - 1);
-    kbias[kb] = kbp ? to_score_units(a, kbp[kc]) : 0.f;
+    kbias[kb] = MODE == kKeys ? to_score_units(a, kbp[kc]) : 0.f;
     if (k >= klen) kbias[kb] = -INFINITY;
     const bool in = kbias[kb] != -INFINITY;
 #pragma unroll
@@ -1061,140 +1242,157 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
   if (kb0 >= klen) t0 = ntq;
   const bool edge_keys = k0 + 32 > klen;
 
-  for (int hg = 0; hg < group; ++hg) {
+  for (int hg = split * heads; hg < (split + 1) * heads; ++hg) {
     if (t0 >= ntq) break;
     const int h = kvh * group + hg;
-    const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
-    const T* dop = (const T*)a.dout.p + b * a.dout.sb + h * a.dout.sh;
-    const long long n = (long long)a.B * a.nh * a.Sq, i0 = ((long long)b * a.nh + h) * a.Sq;
-    Tile<T, D, QT> qr, dr;
-    float st[3] = {INFINITY, 0.f, 0.f};
+    const float* rows = a.rows + row_tile(a, (long long)b * a.nh + h, 0);
+    Tile<T, D, QT> qr((const T*)a.q.p + b * a.q.sb + h * a.q.sh, a.q.ss, a.hd, tid);
+    Tile<T, D, QT> dr((const T*)a.dout.p + b * a.dout.sb + h * a.dout.sh, a.dout.ss, a.hd, tid);
     auto fetch = [&](int t) {
-      qr.load(qp + (long long)t * QT * a.q.ss, a.q.ss, a.Sq - t * QT, a.hd, tid);
-      dr.load(dop + (long long)t * QT * a.dout.ss, a.dout.ss, a.Sq - t * QT, a.hd, tid);
-      if (tid < QT) {
-        const int q = t * QT + tid;
-        const bool in = q < a.Sq;
-        st[0] = in ? a.stat[i0 + q] : INFINITY;
-        st[1] = in ? a.stat[n + i0 + q] : 0.f;
-        st[2] = in ? a.delta[i0 + q] : 0.f;
+      char* img = mem + (t / GROUPS & 1) * 2 * IMG;
+      qr.load(t, a.Sq - t * QT, img, wid);
+      dr.load(t, a.Sq - t * QT, img + IMG, wid);
+      if (wid == 0) {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(rows) + (t * QT / 64) * (long long)kRowStats, 0, kRowStats * 4, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(stl + (t / GROUPS & 1) * kRowStats), 16, lane * 16, 0, 0, 0);
       }
     };
-    auto put = [&](int buf) {
-      char* qimg = smem + buf * 2 * IMG;
-      qr.store(qimg, tid);
-      dr.store(qimg + IMG, tid);
-      if (tid < QT) {
-        float* s = stl + buf * 3 * QT + tid;
-        s[0] = BIAS ? st[0] : st[0] + st[1];
-        s[QT] = st[1];
-        s[2 * QT] = st[2];
-      }
+    auto put = [&](int t) {
+      char* img = mem + (t / GROUPS & 1) * 2 * IMG;
+      qr.put(img);
+      dr.put(img + IMG);
+      loads_done();
     };
-    if (BIAS && a.table) fill_band(a, h, band, tid);     // (the previous head's last barrier has passed)
-    fetch(t0);
-    put(t0 & 1);
+    const int tg = t0 + grp;
+    if (tg < ntq) fetch(tg);
+    if (rel && grp == 0) fill_band(a, h, band, tid);     // (the previous head's last barrier has passed)
+    if (tg < ntq) put(tg);
     __syncthreads();
-    for (int t = t0; t < ntq; ++t) {
-      const char* qimg = smem + (t & 1) * 2 * IMG;
+    for (int t = tg; t - grp < ntq; t += GROUPS) {       // (the groups take turns; all of them keep step)
+      const char* qimg = mem + (t / GROUPS & 1) * 2 * IMG;
       const char* dimg = qimg + IMG;
-      const float* stc = stl + (t & 1) * 3 * QT;
+      const float* stc = stl + (t / GROUPS & 1) * kRowStats + (t * QT & 63);
       const int pos = start + t * QT;                    // position of the tile's first query
-      if (t + 1 < ntq) fetch(t + 1);
-      if (k0 < klen && (!a.causal || k0 <= pos + QT - 1)) {
-        const bool far = BIAS && a.table && (k0 + 31 - pos <= -a.max_dist || k0 - (pos + QT - 1) >= a.right);
+      if (t + GROUPS < ntq) fetch(t + GROUPS);
+      if (t < ntq && k0 < klen && (!a.causal || k0 <= pos + QT - 1)) {
+        const bool far = rel && (k0 + 31 - pos <= -a.max_dist || k0 - (pos + QT - 1) >= a.right);
         const bool edge = a.causal && k0 + 31 > pos;
         float xf = 0.f;
         if (far) xf = k0 < pos ? band[0] : band[band_size(a) - 1];
         const float* at = band + (k0 + fr - pos - 4 * g + a.max_dist + kMargin);   // (query 4 g of block 0, key fr of block 0)
 #pragma unroll
         for (int hf = 0; hf < QT / 32; ++hf) {
-          f32x4 s[2][2], dp[2][2];
-#pragma unroll
-          for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-              const float b0 = BIAS ? kbias[kb] + xf : 0.f;
-              s[ii][kb] = f32x4{b0, b0, b0, b0};
-              dp[ii][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-          if (BIAS && a.table && !far) {
-#pragma unroll
-            for (int j = 0; j < 3; ++j) {                // key block minus query block of the half: -1, 0, 1
-              f32x4 x;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) x[r] = at[(j - 1 - hf * 2) * 16 - r];
-              if (j == 0) s[1][0] += x;
-              if (j == 1) { s[0][0] += x; s[1][1] += x; }
-              if (j == 2) s[0][1] += x;
-            }
-          }
-#pragma unroll
-          for (int ks = 0; ks < DS; ++ks)
-#pragma unroll
-            for (int ii = 0; ii < 2; ++ii) {
-              Frag<T> qfr, dfr;
-              frag_row<ST>(qfr, qimg, (hf * 2 + ii) * 16, ks, lane);
-              frag_row<ST>(dfr, dimg, (hf * 2 + ii) * 16, ks, lane);
-#pragma unroll
-              for (int kb = 0; kb < 2; ++kb) {
-                s[ii][kb] = mma(qfr, kf[kb][ks], s[ii][kb]);
-                dp[ii][kb] = mma(dfr, vf[kb][ks], dp[ii][kb]);
-              }
-            }
-          if (edge || (!BIAS && edge_keys)) {            // with biases a key past the end has -inf already
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-              const int key = k0 + kb * 16 + fr;
-#pragma unroll
-              for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (key >= klen || (a.causal && key > pos + (hf * 2 + ii) * 16 + 4 * g + r)) s[ii][kb][r] = -INFINITY;
-            }
-          }
-          Frag<T> pf[2], dsf[2];
+          f32x4 p[2][2], ds[2][2];
 #pragma unroll
           for (int ii = 0; ii < 2; ++ii) {
             const float* sr = stc + (hf * 2 + ii) * 16 + g * 4;
+            const f32x4 nd = *reinterpret_cast<const f32x4*>(sr + 128);
+            f32x4 s[2], dp[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              const float b0 = MODE == kKeys ? kbias[kb] + xf : MODE == kRel ? xf : 0.f;
+              s[kb] = f32x4{b0, b0, b0, b0};
+              dp[kb] = nd;                               // dP - D comes out of the product
+            }
+            if (rel && !far) {
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[kb][r] += at[(kb - ii - hf * 2) * 16 - r];
+            }
+#pragma unroll
+            for (int ks = 0; ks < DS; ++ks) {
+              Frag<T> qfr, dfr;
+              rd.read_row(qfr, qimg, (hf * 2 + ii) * 16, ks);
+              rd.read_row(dfr, dimg, (hf * 2 + ii) * 16, ks);
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb) {
+                s[kb] = mma(qfr, kf[kb][ks], s[kb]);
+                dp[kb] = mma(dfr, vf[kb][ks], dp[kb]);
+              }
+            }
+            if (edge || (MODE != kKeys && edge_keys)) {  // with key biases a key past the end has -inf already
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb) {
+                // rows of the tile before this one do not see the key
+                const int key = k0 + kb * 16 + fr, first = key >= klen ? QT : a.causal ? key - pos - 4 * g : -QT;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if ((hf * 2 + ii) * 16 + r < first) s[kb][r] = -INFINITY;
+              }
+            }
             const f32x4 mm = *reinterpret_cast<const f32x4*>(sr);
-            const f32x4 ls = *reinterpret_cast<const f32x4*>(sr + QT);
-            const f32x4 de = *reinterpret_cast<const f32x4*>(sr + 2 * QT);
+            f32x4 ls;
+            if (MODE == kKeys) ls = *reinterpret_cast<const f32x4*>(sr + 64);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float p = fexp2(BIAS ? fmaf(s[ii][kb][r] - mm[r], c, -ls[r]) : fmaf(s[ii][kb][r], c, -mm[r]));
-                s[ii][kb][r] = p;
-                dp[ii][kb][r] = p * (dp[ii][kb][r] - de[r]);
+                p[ii][kb][r] = fexp2(MODE == kKeys ? fmaf(s[kb][r] - mm[r], c, -ls[r]) : fmaf(s[kb][r], c, -mm[r]));
+                ds[ii][kb][r] = p[ii][kb][r] * dp[kb][r];
               }
           }
+          Frag<T> pf[2], dsf[2];
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
-            pack(pf[kb], s[0][kb], s[1][kb]);
-            pack(dsf[kb], dp[0][kb], dp[1][kb]);
+            pack(pf[kb], p[0][kb], p[1][kb]);
+            pack(dsf[kb], ds[0][kb], ds[1][kb]);
           }
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
             Frag<T> dot_, qt_;
-            frag_tr<ST>(dot_, dimg, db * 16, hf, lane);
-            frag_tr<ST>(qt_, qimg, db * 16, hf, lane);
+            rd.read_tr(dot_, dimg, db, hf);
+            rd.read_tr(qt_, qimg, db, hf);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
               dv[db][kb] = mma(dot_, pf[kb], dv[db][kb]);
               dk[db][kb] = mma(qt_, dsf[kb], dk[db][kb]);
             }
           }
+          if (D > 64) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (t + 1 < ntq) put((t + 1) & 1);
+      if (t + GROUPS < ntq) put(t + GROUPS);
       __syncthreads();
     }
   }
+  if (GROUPS > 1) {                                     // join: the second group's sums through the images' memory, dK then dV
+    float* oj = reinterpret_cast<float*>(smem) + wid * 32 * D;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      __syncthreads();
+      if (grp == 1) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(oj + ((kb * DB + db) * 64 + lane) * 4) = w ? dv[db][kb] : dk[db][kb];
+      }
+      __syncthreads();
+      if (grp == 0) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(oj + ((kb * DB + db) * 64 + lane) * 4);
+            if (w) dv[db][kb] += x; else dk[db][kb] += x;
+          }
+      }
+    }
+    if (grp == 1) return;
+  }
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
-    const int k = k0 + kb * 16 + fr;
-    if (k < a.Sk) {
+    const int k = opaque(k0 + kb * 16 + fr);             // (the rows' addresses are not for the loop to keep)
+    if (k >= a.Sk) continue;
+    if (a.ksplits > 1) {                                 // [split][2][row][D], joined by dkdv_join_kernel
+      const long long rows = (long long)a.B * a.nkv * a.Sk, row = (long long)bk * a.Sk + k;
+      float* kpart = a.part + ((long long)split * 2 * rows + row) * D;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        *reinterpret_cast<f32x4*>(kpart + db * 16 + g * 4) = dk[db][kb];
+        *reinterpret_cast<f32x4*>(kpart + rows * D + db * 16 + g * 4) = dv[db][kb];
+      }
+    } else {
       T* krow = (T*)a.dk.p + b * a.dk.sb + (long long)k * a.dk.ss + kvh * a.dk.sh;
       T* vrow = (T*)a.dv.p + b * a.dv.sb + (long long)k * a.dv.ss + kvh * a.dv.sh;
 #pragma unroll
@@ -1207,21 +1405,39 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 2 : 1)) void bwd_
   }
 }
 
-// ---- host -----------------------------------------------------------------------------------------------------------
-inline int lds_tiles(int es, int D) {                    // bytes of the two double-buffered tile images
-  const int kt = es == 2 ? 64 : 32;
-  return 4 * kt * (D * es + 16);
+// dk, dv of one key of one key head: the sums over the splits of its query heads. D / 4 lanes a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkdv_join_kernel(Args a) {
+  constexpr int L = D / 4;
+  const long long rows = (long long)a.B * a.nkv * a.Sk, i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / L;
+  const int d = (int)(i - row * L) * 4;
+  if (row >= rows || d >= a.hd) return;
+  const long long bk = row / a.Sk;
+  const int b = (int)(bk / a.nkv), kvh = (int)(bk - (long long)b * a.nkv), k = (int)(row - bk * a.Sk);
+  f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
+  for (int s = 0; s < a.ksplits; ++s) {
+    const float* p = a.part + ((long long)s * 2 * rows + row) * D + d;
+    dk += *reinterpret_cast<const f32x4*>(p);
+    dv += *reinterpret_cast<const f32x4*>(p + rows * D);
+  }
+  store4((T*)a.dk.p + b * a.dk.sb + (long long)k * a.dk.ss + kvh * a.dk.sh + d, dk * a.scale);
+  store4((T*)a.dv.p + b * a.dv.sb + (long long)k * a.dv.ss + kvh * a.dv.sh + d, dv);
 }
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+// bytes of two double-buffered tile images, and of a band
+template <typename T, int D> constexpr int lds_tiles() { return 4 * key_tile<T>() * row_stride<T, D>(); }
+inline int band_floats(const Args& a) { return a.table ? a.max_dist + a.right + 1 + 2 * kMargin : 0; }
 template <typename K>
 inline int set_lds(K kernel, int bytes) {
   if (bytes <= 64 * 1024) return 0;
   return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 template <typename K>
-inline int launch(K kernel, long long blocks, int lds, const Args& a, hipStream_t stream) {
+inline int launch(K kernel, long long blocks, int threads, int lds, const Args& a, hipStream_t stream) {
   const int rc = set_lds(kernel, lds);
   if (rc) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), (size_t)lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)lds, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -1234,54 +1450,100 @@ inline int few_splits(int B, int Sk, int nkv) {
   n = n < most ? n : most;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
-template <typename T, int D, int QB, bool BIAS>
+template <typename T, int D, int QB, int MODE>
 int run_few(const Args& a, hipStream_t stream) {
   constexpr int img = kFewKeys * row_stride<T, D>(), join = QB * 16 * (D + 4) * 4;
   const int lds = 4 * (img > join ? img : join) + 4 * (8 * QB * 16 + (a.table ? a.nh / a.nkv * a.buckets : 0));
-  const int rc = launch(few_kernel<T, D, QB, BIAS>, (long long)a.B * a.nkv * a.splits, lds, a, stream);
+  const int rc = launch(few_kernel<T, D, QB, MODE>, (long long)a.B * a.nkv * a.splits, 256, lds, a, stream);
   if (rc || a.splits == 1) return rc;
-  hipLaunchKernelGGL((few_join_kernel<T, D, BIAS>), dim3((unsigned)(a.B * a.nh * a.Sq)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((few_join_kernel<T, D, MODE>), dim3((unsigned)(a.B * a.nh * a.Sq)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
+// Splits of the dK / dV kernel over the query heads of a key head, so that about three workgroups come to a CU.
+inline int dkdv_splits(int B, int Sk, int nh, int nkv) {
+  const long long n = (long long)B * nkv * ((Sk + kRows - 1) / kRows), group = nh / nkv;
+  for (long long s = 1; s < group; ++s)
+    if (group % s == 0 && n * s >= 768) return (int)s;
+  return (int)group;
+}
 
-template <typename T, int D>
+// Workgroups of eight waves instead of four, whose two halves walk every other tile: for grids that leave the CUs with
+// too few waves to hide a tile's chain of products and exponentials, and for sequences long enough to share out.
+inline bool two_groups(long long blocks, int tiles, int D) { return blocks <= (D <= 64 ? 1024 : 256) && tiles >= 4; }
+
+template <typename T, int D, int MODE, int GROUPS>
+int run_fwd_as(const Args& a, long long n, hipStream_t stream) {
+  const int lds = GROUPS * (lds_tiles<T, D>() + 8 * key_tile<T>()) + 4 * (GROUPS > 1 && band_floats(a) < 1024 ? 1024 : band_floats(a));
+  return launch(fwd_kernel<T, D, MODE, GROUPS>, n, 256 * GROUPS, lds, a, stream);
+}
+template <typename T, int D, int MODE>
 int run_fwd(const Args& a, hipStream_t stream) {
-  const bool bias = a.key_bias || a.table;
-  if (few_queries(a.Sq, a.nh, a.nkv)) {
-    if (a.Sq * (a.nh / a.nkv) <= 16) return bias ? run_few<T, D, 1, true>(a, stream) : run_few<T, D, 1, false>(a, stream);
-    return bias ? run_few<T, D, 2, true>(a, stream) : run_few<T, D, 2, false>(a, stream);
-  }
-  const int nqt = (a.Sq + kRows - 1) / kRows, kt = key_tile<T>();
-  const int band = a.table ? a.max_dist + a.right + 1 + 2 * kMargin : 0;
-  const int lds = lds_tiles(sizeof(T), D) + 4 * (2 * kt + band);
-  const long long n = (long long)a.B * a.nh * nqt;
-  return bias ? launch(fwd_kernel<T, D, true>, n, lds, a, stream) : launch(fwd_kernel<T, D, false>, n, lds, a, stream);
+  if (few_queries(a.Sq, a.nh, a.nkv))
+    return a.Sq * (a.nh / a.nkv) <= 16 ? run_few<T, D, 1, MODE>(a, stream) : run_few<T, D, 2, MODE>(a, stream);
+  const long long n = (long long)a.B * a.nh * ((a.Sq + kRows - 1) / kRows);
+  return two_groups(n, a.Sk / key_tile<T>(), D) ? run_fwd_as<T, D, MODE, 2>(a, n, stream) : run_fwd_as<T, D, MODE, 1>(a, n, stream);
 }
-template <typename T, int D>
+template <typename T, int D, int MODE, int GROUPS>
+int run_dq(const Args& a, long long n, hipStream_t stream) {
+  const int band = band_floats(a);
+  const int lds = GROUPS * (lds_tiles<T, D>() + 8 * key_tile<T>()) + 4 * (band + (a.dtab ? 4 * GROUPS * (band + 2) : 0));
+  return launch(bwd_dq_kernel<T, D, MODE, GROUPS>, n, 256 * GROUPS, lds, a, stream);
+}
+template <typename T, int D, int MODE, int GROUPS>
+int run_dkdv(const Args& a, long long n, hipStream_t stream) {
+  const int lds = GROUPS * (lds_tiles<T, D>() + 8 * kRowStats) + 4 * band_floats(a);
+  return launch(bwd_dkdv_kernel<T, D, MODE, GROUPS>, n, 256 * GROUPS, lds, a, stream);
+}
+constexpr int kMaxLds = 160 * 1024;
+template <typename T, int D, int MODE>
 int run_bwd(const Args& a, hipStream_t stream) {
-  const bool bias = a.key_bias || a.table;
   const int nqt = (a.Sq + kRows - 1) / kRows, nkt = (a.Sk + kRows - 1) / kRows, kt = key_tile<T>();
-  const int band = a.table ? a.max_dist + a.right + 1 + 2 * kMargin : 0;
-  int lds = lds_tiles(sizeof(T), D) + 4 * (2 * kt + band + (a.dtab ? 4 * band + 8 : 0));
-  const long long nq = (long long)a.B * a.nh * nqt, nk = (long long)a.B * a.nkv * nkt;
-  int rc = bias ? launch(bwd_dq_kernel<T, D, true>, nq, lds, a, stream) : launch(bwd_dq_kernel<T, D, false>, nq, lds, a, stream);
+  const long long nq = (long long)a.B * a.nh * nqt, nk = (long long)a.B * a.nkv * nkt * a.ksplits;
+  // (a long band of sums for each of eight waves may not fit)
+  const bool fits = 2 * (lds_tiles<T, D>() + 8 * kt) + 4 * (9 * band_floats(a) + 16) <= kMaxLds;
+  int rc = two_groups(nq, a.Sk / kt, D) && fits ? run_dq<T, D, MODE, 2>(a, nq, stream) : run_dq<T, D, MODE, 1>(a, nq, stream);
   if (rc) return rc;
-  lds = lds_tiles(sizeof(T), D) + 4 * (6 * kt + band);
-  return bias ? launch(bwd_dkdv_kernel<T, D, true>, nk, lds, a, stream) : launch(bwd_dkdv_kernel<T, D, false>, nk, lds, a, stream);
+  rc = two_groups(nk, a.Sq / kt, D) ? run_dkdv<T, D, MODE, 2>(a, nk, stream) : run_dkdv<T, D, MODE, 1>(a, nk, stream);
+  if (rc || a.ksplits == 1) return rc;
+  const long long n = (long long)a.B * a.nkv * a.Sk * (D / 4);
+  hipLaunchKernelGGL((dkdv_join_kernel<T, D>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
 }
-template <typename T>
-int dispatch_fwd(const Args& a, hipStream_t s) {
-  return a.hd <= 32 ? run_fwd<T, 32>(a, s) : a.hd <= 64 ? run_fwd<T, 64>(a, s) : a.hd <= 96 ? run_fwd<T, 96>(a, s) : run_fwd<T, 128>(a, s);
-}
-template <typename T>
-int dispatch_bwd(const Args& a, hipStream_t s) {
-  return a.hd <= 32 ? run_bwd<T, 32>(a, s) : a.hd <= 64 ? run_bwd<T, 64>(a, s) : a.hd <= 96 ? run_bwd<T, 96>(a, s) : run_bwd<T, 128>(a, s);
+template <typename T, int MODE>
+int by_head_size(const Args& a, bool backward, hipStream_t s) {
+  if (a.hd <= 32) return backward ? run_bwd<T, 32, MODE>(a, s) : run_fwd<T, 32, MODE>(a, s);
+  if (a.hd <= 64) return backward ? run_bwd<T, 64, MODE>(a, s) : run_fwd<T, 64, MODE>(a, s);
+  if (a.hd <= 96) return backward ? run_bwd<T, 96, MODE>(a, s) : run_fwd<T, 96, MODE>(a, s);
+  return backward ? run_bwd<T, 128, MODE>(a, s) : run_fwd<T, 128, MODE>(a, s);
 }
 
-int fwd_bf16(const Args& a, hipStream_t s);
-int bwd_bf16(const Args& a, hipStream_t s);
-int fwd_f32(const Args& a, hipStream_t s);
-int bwd_f32(const Args& a, hipStream_t s);
+// one instance of the kernels a source file: (type, mode)
+typedef int (*Run)(const Args& a, bool backward, hipStream_t s);
+int run_bf16_plain(const Args& a, bool backward, hipStream_t s);
+int run_bf16_rel(const Args& a, bool backward, hipStream_t s);
+int run_bf16_keys(const Args& a, bool backward, hipStream_t s);
+int run_f32_plain(const Args& a, bool backward, hipStream_t s);
+int run_f32_rel(const Args& a, bool backward, hipStream_t s);
+int run_f32_keys(const Args& a, bool backward, hipStream_t s);
 
 }  // namespace attn
 }  // namespace dtf
+
+// The kernels of one (type, mode), named one by one: left to the launches in by_head_size, the host pass drops some.
+#define DTF_ATTN_KERNELS(T, D, M)                            \
+  template __global__ void fwd_kernel<T, D, M, 1>(Args);      \
+  template __global__ void fwd_kernel<T, D, M, 2>(Args);      \
+  template __global__ void bwd_dq_kernel<T, D, M, 1>(Args);   \
+  template __global__ void bwd_dq_kernel<T, D, M, 2>(Args);   \
+  template __global__ void bwd_dkdv_kernel<T, D, M, 1>(Args); \
+  template __global__ void bwd_dkdv_kernel<T, D, M, 2>(Args);
+#define DTF_ATTN_INSTANCE(NAME, T, M)                                                   \
+  namespace dtf {                                                                       \
+  namespace attn {                                                                      \
+  DTF_ATTN_KERNELS(T, 32, M)                                                            \
+  DTF_ATTN_KERNELS(T, 64, M)                                                            \
+  DTF_ATTN_KERNELS(T, 96, M)                                                            \
+  DTF_ATTN_KERNELS(T, 128, M)                                                           \
+  int NAME(const Args& a, bool backward, hipStream_t s) { return by_head_size<T, M>(a, backward, s); } \
+  }                                                                                     \
+  }

@@ -11,7 +11,7 @@ namespace {
 enum Word {
   kTensors = 0,          // q k v out dout dq dk dv: pointer and (batch, token, head) strides in elements, four words each
   kKeyBias = 32, kLens, kQStart, kQStart0, kTable, kTableBf16, kBuckets, kMaxDist, kBidirectional,
-  kStat, kDelta, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kPart, kThr   // then the bucket borders
+  kStat, kRowTiles, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kPart, kThr   // then the bucket borders
 };
 
 bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
@@ -35,7 +35,7 @@ bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   a.half = w[kBidirectional] ? a.buckets / 2 : a.buckets;
   a.exact = a.half / 2;
   a.stat = (float*)w[kStat];
-  a.delta = (float*)w[kDelta];
+  a.rows = (float*)w[kRowTiles];
   a.dtab = (float*)w[kDtabParts];
   const long long lim = 1LL << 30;
   for (int i = kB; i <= kHd; ++i)
@@ -44,6 +44,7 @@ bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   a.B = (int)w[kB]; a.Sq = (int)w[kSq]; a.Sk = (int)w[kSk]; a.nh = (int)w[kNh]; a.nkv = (int)w[kNkv]; a.hd = (int)w[kHd];
   a.causal = (int)w[kCausal];
   a.scale = scale;
+  a.inv_scale = 1.f / scale;
   if (!(scale > 0.f) || scale > 1e30f || a.hd % 8 || a.hd > 128 || a.nh % a.nkv) return false;
   if (a.table) {
     a.n_thr = a.half - a.exact - 1;
@@ -65,12 +66,18 @@ bool operands_ok(const attn::Args& a, int size, bool backward) {
     if (t[i]->sb % per16 || t[i]->ss % per16 || t[i]->sh % per16) return false;
     if (t[i]->sb < 0 || t[i]->sh < 0 || t[i]->ss < a.hd || t[i]->ss > (1 << 22)) return false;
   }
-  return !backward || (a.stat && a.delta);
+  return !backward || (a.stat && a.rows && !(reinterpret_cast<uintptr_t>(a.rows) & 15));
+}
+
+attn::Run instance(const attn::Args& a, bool bf16) {
+  if (a.key_bias) return bf16 ? attn::run_bf16_keys : attn::run_f32_keys;
+  if (a.table) return bf16 ? attn::run_bf16_rel : attn::run_f32_rel;
+  return bf16 ? attn::run_bf16_plain : attn::run_f32_plain;
 }
 
 bool grid_ok(const attn::Args& a) {
   const long long q = (long long)a.B * a.nh * ((a.Sq + attn::kRows - 1) / attn::kRows);
-  const long long k = (long long)a.B * a.nkv * ((a.Sk + attn::kRows - 1) / attn::kRows);
+  const long long k = (long long)a.B * a.nh * ((a.Sk + attn::kRows - 1) / attn::kRows);
   return q < (1LL << 31) / 256 && k < (1LL << 31) / 256;
 }
 
@@ -96,6 +103,10 @@ __global__ __launch_bounds__(256) void dtab_finish_kernel(const float* __restric
 
 }  // namespace
 
+// Splits of the backward pass over the query heads of a key head. More than one: it needs a scratch of splits * 2 * B *
+// nkv * Sk * (hd rounded up to 32) floats.
+DTF_API int dtf_attention_bwd_splits(int B, int Sk, int nh, int nkv) { return nkv > 0 ? attn::dkdv_splits(B, Sk, nh, nkv) : 1; }
+
 // Key splits of the forward pass. More than one: it needs a scratch of splits * B * nh * Sq * (hd rounded up to 32, + 2)
 // floats.
 DTF_API int dtf_attention_splits(int B, int Sq, int Sk, int nh, int nkv) {
@@ -111,10 +122,10 @@ DTF_API int dtf_attention_fwd(const long long* words, int n_words, float scale, 
   a.splits = dtf_attention_splits(a.B, a.Sq, a.Sk, a.nh, a.nkv);
   a.part = (float*)words[kPart];
   if (a.splits > 1 && !a.part) return -5;
-  return bf16 ? attn::fwd_bf16(a, stream) : attn::fwd_f32(a, stream);
+  return instance(a, bf16)(a, false, stream);
 }
 
-// dtab parts: fp32 [B * ceil(Sq / 128)][nh][buckets] scratch; dtab out: [buckets, nh] in the table's type. Both or neither.
+// row tiles: fp32 scratch of B * nh * ceil(Sq / 128) * 512. dtab parts: fp32 [B * ceil(Sq / 128)][nh][buckets] scratch; dtab out: [buckets, nh] in the table's type. Both or neither.
 DTF_API int dtf_attention_bwd(const long long* words, int n_words, float scale, hipStream_t stream) {
   attn::Args a = {};
   if (!unpack(words, n_words, scale, a)) return -1;
@@ -123,7 +134,10 @@ DTF_API int dtf_attention_bwd(const long long* words, int n_words, float scale, 
   if (!grid_ok(a)) return -3;
   void* out = (void*)words[kDtabOut];
   if ((a.dtab != nullptr) != (out != nullptr) || (out && !a.table)) return -4;
-  const int rc = bf16 ? attn::bwd_bf16(a, stream) : attn::bwd_f32(a, stream);
+  a.ksplits = dtf_attention_bwd_splits(a.B, a.Sk, a.nh, a.nkv);
+  a.part = (float*)words[kPart];
+  if (a.ksplits > 1 && !a.part) return -5;
+  const int rc = instance(a, bf16)(a, true, stream);
   if (rc || !a.dtab) return rc;
   hipLaunchKernelGGL(dtab_finish_kernel, dim3(a.nh), dim3(256), 0, stream, a.dtab, out,
                      a.B * ((a.Sq + attn::kRows - 1) / attn::kRows), a.nh, a.buckets, a.table_bf16);

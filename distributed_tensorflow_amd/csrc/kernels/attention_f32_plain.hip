@@ -1,0 +1,4 @@
+// Instances of the general attention kernels (attention.h): f32, no bias.
+#include "attention.h"
+
+DTF_ATTN_INSTANCE(run_f32_plain, float, kPlain)

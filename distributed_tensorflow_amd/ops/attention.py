@@ -271,20 +271,25 @@ class _GeneralFn(torch.autograd.Function):
             dk, dv = torch.empty(k.shape, dtype=dt, device=dev), torch.empty(k.shape, dtype=dt, device=dev)
             grads = (*_dense(dq.data_ptr(), Sq, nh, hd), *_dense(dk.data_ptr(), Sk, nkv, hd),
                      *_dense(dv.data_ptr(), Sk, nkv, hd))
-        n = B * nh * Sq
         if table is not None and ctx.needs_input_grad[3]:
             dtable = torch.empty(ctx.table_like[0], dtype=ctx.table_like[1], device=dev)
-        if n == 0 or Sk == 0:
+        if out.numel() == 0 or Sk == 0:
             for t in (dq, dk, dv, dtable):
                 if t is not None:
                     t.zero_()
             return dq, dk, dv, dtable, None, None, None, None, None
-        # rowsum(dO * O), then the partial sums of the table's gradient
+        # statistics of the queries for the dK / dV kernel, then the partial sums of the table's gradient
+        n = B * nh * -(-Sq // 128) * 512
         scratch = torch.empty(n + (0 if dtable is None else B * -(-Sq // 128) * dtable.numel()), dtype=torch.float32, device=dev)
         p = scratch.data_ptr()
+        part, splits = 0, 1
+        if nh > nkv:                               # grouped heads: dK and dV may be summed in splits of the group
+            splits = _lib.kernels().dtf_attention_bwd_splits(B, Sk, nh, nkv)
+            if splits > 1:
+                part = torch.empty(splits * 2 * B * nkv * Sk * (-(-hd // 32) * 32), dtype=torch.float32, device=dev)
         dout, dw = _usable(dout)
         _call("dtf_attention_bwd", (*words[:16], *dw, *grads, *words[32:42], p, *((0, 0) if dtable is None else
-              (p + 4 * n, dtable.data_ptr())), *words[45:]), ctx.scale, q)
+              (p + 4 * n, dtable.data_ptr())), *words[45:53], part.data_ptr() if splits > 1 else 0, *words[54:]), ctx.scale, q)
         return dq, dk, dv, dtable, None, None, None, None, None
 
 
