@@ -11,7 +11,7 @@ namespace {
 enum Word {
   kTensors = 0,          // q k v out dout dq dk dv: pointer and (batch, token, head) strides in elements, four words each
   kKeyBias = 32, kLens, kQStart, kQStart0, kTable, kTableBf16, kBuckets, kMaxDist, kBidirectional,
-  kStat, kRowTiles, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kPart, kThr   // then the bucket borders
+  kStat, kRowTiles, kDtabParts, kDtabOut, kB, kSq, kSk, kNh, kNkv, kHd, kCausal, kBf16, kPart, kFine, kThr   // then the bucket borders
 };
 
 bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
@@ -43,6 +43,8 @@ bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   if (w[kQStart0] > lim || w[kQStart0] < -lim) return false;
   a.B = (int)w[kB]; a.Sq = (int)w[kSq]; a.Sk = (int)w[kSk]; a.nh = (int)w[kNh]; a.nkv = (int)w[kNkv]; a.hd = (int)w[kHd];
   a.causal = (int)w[kCausal];
+  a.part = (float*)w[kPart];
+  a.fine = (unsigned char*)w[kFine];
   a.scale = scale;
   a.inv_scale = 1.f / scale;
   if (!(scale > 0.f) || scale > 1e30f || a.hd % 8 || a.hd > 128 || a.nh % a.nkv) return false;
@@ -66,6 +68,7 @@ bool operands_ok(const attn::Args& a, int size, bool backward) {
     if (t[i]->sb % per16 || t[i]->ss % per16 || t[i]->sh % per16) return false;
     if (t[i]->sb < 0 || t[i]->sh < 0 || t[i]->ss < a.hd || t[i]->ss > (1 << 22)) return false;
   }
+  if (reinterpret_cast<uintptr_t>(a.fine) & 7 || (backward && size == 2 && !a.fine)) return false;
   return !backward || (a.stat && a.rows && !(reinterpret_cast<uintptr_t>(a.rows) & 15));
 }
 
@@ -120,7 +123,6 @@ DTF_API int dtf_attention_fwd(const long long* words, int n_words, float scale, 
   if (!operands_ok(a, bf16 ? 2 : 4, false)) return -2;
   if (!grid_ok(a)) return -3;
   a.splits = dtf_attention_splits(a.B, a.Sq, a.Sk, a.nh, a.nkv);
-  a.part = (float*)words[kPart];
   if (a.splits > 1 && !a.part) return -5;
   return instance(a, bf16)(a, false, stream);
 }
@@ -135,7 +137,6 @@ DTF_API int dtf_attention_bwd(const long long* words, int n_words, float scale, 
   void* out = (void*)words[kDtabOut];
   if ((a.dtab != nullptr) != (out != nullptr) || (out && !a.table)) return -4;
   a.ksplits = dtf_attention_bwd_splits(a.B, a.Sk, a.nh, a.nkv);
-  a.part = (float*)words[kPart];
   if (a.ksplits > 1 && !a.part) return -5;
   const int rc = instance(a, bf16)(a, true, stream);
   if (rc || !a.dtab) return rc;

@@ -207,7 +207,7 @@ def _dense(p, S, n, hd):
     return p, S * n * hd, n * hd, hd
 
 
-def _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat):
+def _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat, fine):
     """(out, q, k, v as the kernels read them, table, words of the call)."""
     causal, scale, start0, max_distance, bidirectional = opts
     q, qw = _usable(q)
@@ -235,7 +235,7 @@ def _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat):
              0 if key_bias is None else key_bias.data_ptr(), 0 if lens is None else lens.data_ptr(),
              0 if starts is None else starts.data_ptr(), start0, *rel, max_distance, int(bidirectional),
              0 if stat is None else stat.data_ptr(), 0, 0, 0, B, Sq, Sk, nh, nkv, hd, int(causal), bf16,
-             part.data_ptr() if splits > 1 else 0, *borders)
+             part.data_ptr() if splits > 1 else 0, 0 if fine is None else fine.data_ptr(), *borders)
     if Sk == 0:
         out.zero_()
     elif out.numel():
@@ -251,16 +251,20 @@ class _GeneralFn(torch.autograd.Function):
         B, Sq, n = q.shape[:3]
         stat = torch.empty(2, B, n - 2 * nkv if k is None else n, Sq, dtype=torch.float32, device=q.device)
         ctx.table_like = None if table is None else (table.shape, table.dtype)
-        out, q, k, v, table, ctx.words = _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat)
+        # the bits of the output that bfloat16 cuts off, for the backward pass's rowsum(dO * O)
+        fine = None
+        if q.dtype == torch.bfloat16:
+            fine = torch.empty(B, Sq, n - 2 * nkv if k is None else n, q.shape[3], dtype=torch.uint8, device=q.device)
+        out, q, k, v, table, ctx.words = _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat, fine)
         ctx.scale = opts[1]
         # (the words point into these)
-        ctx.save_for_backward(q, k, v, table, key_bias, lens, starts, out, stat)
+        ctx.save_for_backward(q, k, v, table, key_bias, lens, starts, stat, fine, out)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, *_, out, _ = ctx.saved_tensors
+        q, k, v, table, *_, out = ctx.saved_tensors
         words, dev, dt = ctx.words, q.device, q.dtype
         B, Sq, Sk, nh, nkv, hd = words[45:51]
         dq = torch.empty(q.shape, dtype=dt, device=dev)
@@ -367,7 +371,7 @@ def _general(q, k, v, nkv, key_bias, causal, scale, key_lengths, q_start, rel_ta
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad))
                                     or (rel_table is not None and rel_table.requires_grad)):
         return _GeneralFn.apply(q, k, v, rel_table, key_bias, lens, starts, nkv, opts)
-    return _forward(q, k, v, rel_table, key_bias, lens, starts, nkv, opts, None)[0]
+    return _forward(q, k, v, rel_table, key_bias, lens, starts, nkv, opts, None, None)[0]
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_bias: torch.Tensor | None = None, *,
