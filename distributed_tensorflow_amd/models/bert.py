@@ -9,6 +9,12 @@ decoder (tied to the word embeddings) feeds the fused softmax-cross-entropy over
 Input ``x``: ``int64 [B, S]`` token ids, or ``[B, S + P]`` where the last ``P`` columns are the
 positions to predict (the MLM head then scores only those, as the original pre-training does
 with ``max_predictions_per_seq``). Output: logits ``[B*S or B*P, vocab]``.
+
+``rel_buckets > 0`` replaces the position embeddings by a learned relative position bias: one table
+``[rel_buckets, heads]`` that every layer's attention adds to its scores (``ops/relative_bias.py``), so
+a sequence may have any length. ``key_lengths[B]`` ends each sequence of a padded batch. Both run the
+general fused attention. ``Bert.score`` gives the log probabilities of given tokens at the scored
+positions, with entropy and the best alternatives.
 """
 from __future__ import annotations
 
@@ -21,6 +27,7 @@ from ..ops import attention as attn_ops
 from ..ops import dense as dense_ops
 from ..ops import embedding as emb_ops
 from ..ops import layernorm as ln_ops
+from ..ops.softmax_ce import TokenLogProbs, token_log_probs
 
 
 class Linear(nn.Module):
@@ -76,11 +83,12 @@ class EncoderLayer(nn.Module):
         self.ffn2 = Linear(ffn, h)
         self.ln2 = LayerNorm(h)
 
-    def forward(self, x, key_bias=None):
+    def forward(self, x, key_bias=None, **attention):
+        """``attention``: options of :func:`ops.attention.self_attention`."""
         B, S, H = x.shape
         # the aliases carry the residual branches' gradients into the data-gradient GEMM epilogues
         qkv, xr = dense_ops.linear_fork(x, self.qkv.weight, self.qkv.bias)
-        ctxv = attn_ops.self_attention(qkv.view(B, S, 3, self.heads, H // self.heads), key_bias).view(B, S, H)
+        ctxv = attn_ops.self_attention(qkv.view(B, S, 3, self.heads, H // self.heads), key_bias, **attention).view(B, S, H)
         x = self.ln1(self.proj(ctxv), residual=xr)
         f, xr = dense_ops.ffn_fork(x, self.ffn1.weight, self.ffn1.bias, self.ffn2.weight, self.ffn2.bias)
         return self.ln2(f, residual=xr)
@@ -91,11 +99,17 @@ class Bert(Model):
     input_layout = "tokens"
 
     def __init__(self, vocab: int = 30522, hidden: int = 768, layers: int = 12, heads: int = 12, ffn: int = 3072,
-                 max_pos: int = 512, type_vocab: int = 2, seq_len: int | None = None):
+                 max_pos: int = 512, type_vocab: int = 2, seq_len: int | None = None, rel_buckets: int = 0,
+                 rel_max_distance: int = 128):
         super().__init__()
         self.vocab, self.hidden, self.seq_len = vocab, hidden, seq_len
+        self.rel_max_distance = rel_max_distance
         self.word = nn.Parameter(torch.empty(vocab, hidden).normal_(0, 0.02))
-        self.pos = nn.Parameter(torch.empty(max_pos, hidden).normal_(0, 0.02))
+        self.pos = self.rel = None
+        if rel_buckets:
+            self.rel = nn.Parameter(torch.empty(rel_buckets, heads).normal_(0, 0.02))
+        else:
+            self.pos = nn.Parameter(torch.empty(max_pos, hidden).normal_(0, 0.02))
         self.typ = nn.Parameter(torch.empty(type_vocab, hidden).normal_(0, 0.02))
         self.emb_ln = LayerNorm(hidden)
         self.layers = nn.ModuleList([EncoderLayer(hidden, heads, ffn) for _ in range(layers)])
@@ -106,14 +120,19 @@ class Bert(Model):
     def prepare_input(self, x):
         return x
 
-    def forward(self, x, logits: bool = False):
+    def forward(self, x, logits: bool = False, key_lengths: torch.Tensor | None = None):
         S = self.seq_len if (self.seq_len is not None and x.shape[1] > self.seq_len) else x.shape[1]
         ids, positions = x[:, :S], (x[:, S:] if x.shape[1] > S else None)
         B = ids.shape[0]
         h = emb_ops.embedding(self.word, ids, self.pos, self.typ)
         h = self.emb_ln(h)
+        options = {}
+        if self.rel is not None:
+            options.update(rel_table=self.rel, rel_max_distance=self.rel_max_distance)
+        if key_lengths is not None:
+            options["key_lengths"] = key_lengths
         for l in self.layers:
-            h = l(h)
+            h = l(h, **options)
         if positions is not None:
             idx = (positions + torch.arange(B, device=x.device)[:, None] * S).reshape(-1)
             h = h.reshape(B * S, -1).index_select(0, idx)
@@ -122,6 +141,12 @@ class Bert(Model):
         h = self.head_ln(self.head_dense(h))
         out = dense_ops.linear(h, self.word, self.decoder_bias)    # decoder tied to the word embeddings
         return out if logits else torch.softmax(out.float(), dim=-1)
+
+    @torch.no_grad()
+    def score(self, x, tokens, top: int = 0, key_lengths: torch.Tensor | None = None) -> TokenLogProbs:
+        """Log probability of ``tokens`` (one for each row of logits, below 0: none), the entropy there and the ``top``
+        best alternatives, in one pass over the logits."""
+        return token_log_probs(self(x, logits=True, key_lengths=key_lengths), tokens.reshape(-1), top)
 
 
 def bert_base(seq_len: int = 512, **kw) -> Bert:

@@ -393,3 +393,134 @@ def test_token_log_probs_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, run(leaf.detach().clone().requires_grad_()))), i
+
+
+# ------------------------------------------------------------------------------------------------ large grids, head splits
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cfg", [(40, 260, 260, 32, 32, 8, False), (66, 300, 129, 16, 4, 16, True), (260, 33, 300, 8, 8, 24, False)], ids=str)
+@pytest.mark.parametrize("rel", [0, 16])
+def test_attention_with_a_grid_that_fills_the_chip(dt, cfg, rel):
+    """Small grids run workgroups of two halves; these run the single ones over several tiles. Two distinct sequences,
+    repeated: every copy is bitwise the same (the table's gradient aside, which sums them), and right."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    B, Sq, Sk, nh, nkv, hd, causal = cfg
+    q, k, v, do, table = _inputs(2, Sq, Sk, nh, nkv, hd, dt, rel, seed=9)
+    val, tol = O.attention(q, k, v, do, causal=causal, rel_table=table, rel_max_distance=40)
+    big = [t.to(DEV).repeat(B // 2, 1, 1, 1).requires_grad_() for t in (q, k, v)]
+    tab = None if table is None else table.to(DEV).requires_grad_()
+    out = attention(*big, causal=causal, rel_table=tab, rel_max_distance=40)
+    got = torch.autograd.grad(out, big + ([tab] if rel else []), do.to(DEV).repeat(B // 2, 1, 1, 1))
+    for n, t in zip(("out", "dq", "dk", "dv"), (out, *got)):
+        assert torch.equal(t, t[:2].repeat(B // 2, 1, 1, 1)), n
+        O.check(n, t[:2], val[n], tol[n])
+    if rel:                                   # (B / 2 times the sums; the bound's own rounding is already one of the result)
+        O.check("dtable", got[3], val["dtable"] * (B // 2), tol["dtable"] * (B // 2))
+
+
+@pytest.mark.parametrize("shape", [(1, 300, 300, 8, 1, 64), (1, 200, 333, 12, 2, 128), (2, 140, 140, 6, 2, 32)], ids=str)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+def test_attention_sums_shared_heads_over_splits(shape, causal):
+    """Many query heads to a key head and few key heads: dK and dV are summed in parts and joined."""
+    q, k, v, do, table = _inputs(*shape, BF16, 16, seed=5)
+    _compare(q, k, v, do, table, causal=causal, rel_max_distance=60)
+
+
+# ------------------------------------------------------------------------------------------------ together, in the model
+def _tiny(device, dtype, seed=0):
+    from distributed_tensorflow_amd.models.bert import bert_tiny
+    torch.manual_seed(seed)
+    return bert_tiny(seq_len=77, vocab=1000, rel_buckets=16, rel_max_distance=50).to(device=device, dtype=dtype)
+
+
+def test_bert_with_relative_positions_matches_the_cpu_model():
+    """The fp32 model on the GPU (general attention with the relative bias and padded batches, scoring) against the same
+    weights on the CPU in fp32: two layers of sums of at most 1024 terms, both sides off by at most some 1024 * 2^-24 of
+    the largest magnitude each."""
+    from distributed_tensorflow_amd.models.bert import synthetic_mlm_batch
+    x, y = synthetic_mlm_batch(3, 77, 1000, "cpu", n_pred=9)
+    n = torch.tensor([77, 40, 1], dtype=torch.int32)
+    res = []
+    for dev in ("cpu", DEV):
+        m = _tiny("cpu", FP32).to(dev)
+        logits = m(x.to(dev), logits=True, key_lengths=n.to(dev))
+        (logits.float().logsumexp(1).sum() - logits[torch.arange(27), y].sum()).backward()
+        s = m.score(x.to(dev), y.to(dev), 5, key_lengths=n.to(dev))
+        res.append((logits, m.rel.grad, m.layers[0].qkv.weight.grad, m.word.grad, s.logp, s.entropy, s.top_logp))
+    for a, b in zip(*res):
+        a, b = a.detach(), b.detach().cpu()
+        assert float((a - b).abs().max()) <= 2 * 1024 * O.U32 * 8 * float(a.abs().max())
+
+
+def test_bert_with_relative_positions_trains_in_bf16_and_in_a_graph():
+    """Training steps of the strategy, eager and captured: the same losses and weights to the bit, finite, and the table
+    moves."""
+    from distributed_tensorflow_amd.comm.backend import Comm
+    from distributed_tensorflow_amd.engine.optimizer import Adam
+    from distributed_tensorflow_amd.engine.replica import TrainConfig
+    from distributed_tensorflow_amd.models.bert import synthetic_mlm_batch
+    from distributed_tensorflow_amd.parallel.mirrored import MirroredStrategy
+    x, y = synthetic_mlm_batch(6, 77, 1000, DEV, n_pred=9)
+    runs = []
+    for graph in (False, True):
+        cfg = TrainConfig(loss="mlm", param_dtype=BF16, grad_dtype=BF16, graph=graph)
+        st = MirroredStrategy(_tiny("cpu", FP32), Comm(0, 1, torch.device(DEV)), cfg, optimizer=Adam(1e-3))
+        before = st.replica.model.rel.detach().clone()
+        step = st.step_callable() if graph else st.train_step
+        losses = [float(step(x, y)) for _ in range(10)]
+        assert all(math.isfinite(v) for v in losses) and not torch.equal(before, st.replica.model.rel)
+        runs.append((losses, st.flat.master.clone()))
+    assert runs[0][0] == pytest.approx(runs[1][0], rel=1e-6)
+    assert torch.equal(runs[0][1], runs[1][1])
+
+
+def test_operators_in_two_graphs_and_on_two_streams_at_once():
+    """Two captured passes that are replayed in turn and two streams at a time: no call shares a workspace with another."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    from distributed_tensorflow_amd.ops.softmax_ce import token_log_probs
+
+    def make(seed):
+        q, k, v, do, table = (t.to(DEV) for t in _inputs(2, 200, 200, 4, 2, 64, BF16, 32, seed=seed))
+        x = torch.randn(60, 5000, device=DEV, generator=torch.Generator(DEV).manual_seed(seed)).to(BF16)
+        tok = torch.randint(0, 5000, (60,), device=DEV)
+        cache = [torch.randn(2, n, h, 64, device=DEV).to(BF16) for n, h in ((1, 8), (3000, 2), (3000, 2))]
+
+        def run():
+            leaves = [t.detach().requires_grad_() for t in (q, k, v, table)]
+            out = attention(*leaves[:3], rel_table=leaves[3], causal=True)
+            grads = torch.autograd.grad(out, leaves, do)
+            t = table.detach().requires_grad_()
+            bias = relative_bias(t, 200, 200)
+            dt, = torch.autograd.grad(bias, t, bias.detach())
+            lx = x.detach().requires_grad_()
+            r = token_log_probs(lx, tok, 4)
+            dx, = torch.autograd.grad(r.logp.sum(), lx)
+            return [out.detach(), *grads, bias.detach(), dt, *[z.detach() for z in r], dx, attention(*cache)]
+        return run
+
+    runs = [make(1), make(2)]
+    want = [[t.clone() for t in r()] for r in runs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = runs[i]()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+    del got
+    graphs, outs = [], []
+    for r in runs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(r())
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        runs[0]()
+    torch.cuda.synchronize()
+    for g, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))

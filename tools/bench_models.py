@@ -1,6 +1,6 @@
 """Single-GPU training throughput of the non-headline model configurations.
 
-usage: python tools/bench_models.py [bert|resnet20|mlp|widedeep ...] [--steps 10]
+usage: python tools/bench_models.py [bert|bert_relative|resnet20|mlp|widedeep ...] [--steps 10]
 """
 import argparse
 import json
@@ -57,6 +57,26 @@ def main():
         except Exception as e:  # a step that cannot be captured is reported, not fatal
             out.append({"model": "bert-base-mlm-seq512", "hip_graph": True, "error": str(e)[:300]})
             print(out[-1], flush=True)
+        del st
+    if "bert_relative" in a.models:              # relative position bias instead of position embeddings, and scoring
+        from distributed_tensorflow_amd.models.bert import bert_base, synthetic_mlm_batch
+        torch.manual_seed(0)
+        cfg = TrainConfig(loss="mlm", param_dtype=torch.bfloat16, grad_dtype=torch.bfloat16)
+        st = MirroredStrategy(bert_base(512, rel_buckets=32), comm, cfg, optimizer=Adam(learning_rate=1e-4))
+        x, y = synthetic_mlm_batch(a.bert_batch, 512, 30522, DEV, n_pred=80)
+        out.append(run("bert-base-relative-mlm-seq512", st, x, y, a.steps, a.warmup, a.bert_batch, "sequences_per_s"))
+        model = st.replica.model
+        for _ in range(a.warmup):
+            model.score(x, y, top=5)
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(a.steps):
+            r = model.score(x, y, top=5)
+        torch.cuda.synchronize()
+        dt = (time.perf_counter() - t0) / a.steps
+        out.append({"model": "bert-base-relative-score", "ms_per_pass": round(dt * 1e3, 3),
+                    "sequences_per_s": round(a.bert_batch / dt, 1), "mean_logp": float(r.logp.mean())})
+        print(json.dumps(out[-1]), flush=True)
         del st
     if "resnet20" in a.models:
         from distributed_tensorflow_amd.models.resnet import resnet20
