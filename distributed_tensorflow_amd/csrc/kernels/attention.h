@@ -181,10 +181,11 @@ __device__ __forceinline__ unsigned finer(float o) {
   const int d = (int)(((u + 0x80u) >> 8) - b);
   return (unsigned)(d > 127 ? 127 : d) & 0xffu;
 }
-__device__ __forceinline__ void store_finer(const Args& a, int b, int q, int h, int d, const f32x4& o) {
-  if (!a.fine) return;
-  const unsigned w = finer(o[0]) | finer(o[1]) << 8 | finer(o[2]) << 16 | finer(o[3]) << 24;
-  *reinterpret_cast<unsigned*>(a.fine + (((long long)b * a.Sq + q) * a.nh + h) * a.hd + d) = w;
+__device__ __forceinline__ unsigned finer4(const f32x4& o) {
+  return finer(o[0]) | finer(o[1]) << 8 | finer(o[2]) << 16 | finer(o[3]) << 24;
+}
+__device__ __forceinline__ unsigned char* fine_row(const Args& a, int b, int q, int h) {
+  return a.fine + (((long long)b * a.Sq + q) * a.nh + h) * a.hd;
 }
 // dO . O over 8 elements, O with the bits of `fine`
 __device__ __forceinline__ float dot_fine(const Frag<unsigned short>& dout, const Frag<unsigned short>& o, u32x2_t fine, float s) {
@@ -217,6 +218,37 @@ __device__ __forceinline__ float dot(const Frag<float>& a, const Frag<float>& b,
 }
 __device__ __forceinline__ void store4(unsigned short* p, const f32x4& v) { store4_bf16(p, v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
+
+// Results leave the accumulators with 4 consecutive elements of block 2 p in a lane and 4 of block 2 p + 1, 16 apart. Two
+// swaps between lane groups make that 8 consecutive ones, at 32 p + 8 g: a row's 64 (fp32: 128) bytes go out at once instead
+// of in pieces of 8 or 16. x: lane groups' four 0, 1, 2, 3, y: 4, 5, 6, 7; after it x: 0, 2, 4, 6 and y: 1, 3, 5, 7.
+__device__ __forceinline__ void gather8(unsigned& x, unsigned& y) {
+  const u32x2_t h = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(x, y, false, false));
+  const unsigned a = h[0], b = h[1];
+  const u32x2_t r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a, b, false, false));
+  x = r[0];
+  y = r[1];
+}
+__device__ __forceinline__ void store_pair(unsigned short* row, int p, int g, int hd, const f32x4& v0, const f32x4& v1) {
+  unsigned x0 = pack_bf16x2(v0[0], v0[1]), x1 = pack_bf16x2(v0[2], v0[3]);
+  unsigned y0 = pack_bf16x2(v1[0], v1[1]), y1 = pack_bf16x2(v1[2], v1[3]);
+  gather8(x0, y0);
+  gather8(x1, y1);
+  if (p * 32 + g * 8 < hd) *reinterpret_cast<u32x4_t*>(row + p * 32 + g * 8) = u32x4_t{x0, x1, y0, y1};
+}
+__device__ __forceinline__ void store_pair(float* row, int p, int g, int hd, const f32x4& v0, const f32x4& v1) {
+  u32x4_t x, y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned a = __float_as_uint(v0[i]), b = __float_as_uint(v1[i]);
+    gather8(a, b);
+    x[i] = a;
+    y[i] = b;
+  }
+  if (p * 32 + g * 8 >= hd) return;
+  *reinterpret_cast<u32x4_t*>(row + p * 32 + g * 8) = x;
+  *reinterpret_cast<u32x4_t*>(row + p * 32 + g * 8 + 4) = y;
+}
 
 // over the 4 lanes that share lane & 15
 __device__ __forceinline__ float group_max(float v) {
@@ -625,14 +657,19 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
     const int q = q0 + qb * 16 + fr;
     const float lt = l[qb];
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    if (q < a.Sq) {
-      T* row = (T*)a.out.p + b * a.out.sb + (long long)q * a.out.ss + h * a.out.sh;
+    T* row = (T*)a.out.p + b * a.out.sb + (long long)q * a.out.ss + h * a.out.sh;
+    const int hd = q < a.Sq ? a.hd : 0;                 // (every lane takes part in the swaps)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-        if (db * 16 + g * 4 < a.hd) {
-          store4(row + db * 16 + g * 4, o[db][qb] * inv);
-          if (sizeof(T) == 2) store_finer(a, b, q, h, db * 16 + g * 4, o[db][qb] * inv);
-        }
+    for (int p = 0; p < DB / 2; ++p) {
+      const f32x4 v0 = o[2 * p][qb] * inv, v1 = o[2 * p + 1][qb] * inv;
+      store_pair(row, p, g, hd, v0, v1);
+      if (sizeof(T) == 2 && a.fine) {
+        unsigned x = finer4(v0), y = finer4(v1);
+        gather8(x, y);
+        if (p * 32 + g * 8 < hd) *reinterpret_cast<u32x2_t*>(fine_row(a, b, q, h) + p * 32 + g * 8) = u32x2_t{x, y};
+      }
+    }
+    if (q < a.Sq) {
       if (g == 0 && a.stat) {
         const long long i = ((long long)b * a.nh + h) * a.Sq + q, n = (long long)a.B * a.nh * a.Sq;
         a.stat[i] = lt == 0.f ? INFINITY : m[qb];       // +inf: exp2(t - inf) = 0 for a row with nothing in it
@@ -659,7 +696,7 @@ __device__ __forceinline__ void few_store(const Args& a, int b, int kvh, int gro
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   if (d < a.hd) {
     store4((T*)a.out.p + b * a.out.sb + (long long)i * a.out.ss + h * a.out.sh + d, acc * inv);
-    if (sizeof(T) == 2) store_finer(a, b, i, h, d, acc * inv);
+    if (sizeof(T) == 2 && a.fine) *reinterpret_cast<unsigned*>(fine_row(a, b, i, h) + d) = finer4(acc * inv);
   }
   if (d == 0 && a.stat) {
     const long long at = ((long long)b * a.nh + h) * a.Sq + i, n = (long long)a.B * a.nh * a.Sq;
@@ -1007,7 +1044,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
       frag_global(of, op + (long long)qc * a.out.ss, e, e < a.hd);
       if constexpr (sizeof(T) == 2) {
         u32x2_t fine = {0u, 0u};
-        if (e < a.hd) fine = *reinterpret_cast<const u32x2_t*>(a.fine + (((long long)b * a.Sq + qc) * a.nh + h) * a.hd + e);
+        if (e < a.hd) fine = *reinterpret_cast<const u32x2_t*>(fine_row(a, b, qc, h) + e);
         part = dot_fine(dof[qb][ks], of, fine, part);
       } else {
         part = dot(of, dof[qb][ks], part);
@@ -1198,11 +1235,10 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const int q = opaque(q0 + qb * 16 + fr);             // (the rows' addresses are not for the loop to keep)
-    if (q < a.Sq && grp == 0) {
-      T* row = (T*)a.dq.p + b * a.dq.sb + (long long)q * a.dq.ss + h * a.dq.sh;
+    T* row = (T*)a.dq.p + b * a.dq.sb + (long long)q * a.dq.ss + h * a.dq.sh;
+    if (grp == 0) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-        if (db * 16 + g * 4 < a.hd) store4(row + db * 16 + g * 4, dq[db][qb] * a.scale);
+      for (int p = 0; p < DB / 2; ++p) store_pair(row, p, g, q < a.Sq ? a.hd : 0, dq[2 * p][qb] * a.scale, dq[2 * p + 1][qb] * a.scale);
     }
   }
   if (want_tab) {
@@ -1427,8 +1463,8 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
     const int k = opaque(k0 + kb * 16 + fr);             // (the rows' addresses are not for the loop to keep)
-    if (k >= a.Sk) continue;
     if (a.ksplits > 1) {                                 // [split][2][row][D], joined by dkdv_join_kernel
+      if (k >= a.Sk) continue;
       const long long rows = (long long)a.B * a.nkv * a.Sk, row = (long long)bk * a.Sk + k;
       float* kpart = a.part + ((long long)split * 2 * rows + row) * D;
 #pragma unroll
@@ -1439,12 +1475,12 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
     } else {
       T* krow = (T*)a.dk.p + b * a.dk.sb + (long long)k * a.dk.ss + kvh * a.dk.sh;
       T* vrow = (T*)a.dv.p + b * a.dv.sb + (long long)k * a.dv.ss + kvh * a.dv.sh;
+      const int hd = k < a.Sk ? a.hd : 0;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-        if (db * 16 + g * 4 < a.hd) {
-          store4(krow + db * 16 + g * 4, dk[db][kb] * a.scale);
-          store4(vrow + db * 16 + g * 4, dv[db][kb]);
-        }
+      for (int p = 0; p < DB / 2; ++p) {
+        store_pair(krow, p, g, hd, dk[2 * p][kb] * a.scale, dk[2 * p + 1][kb] * a.scale);
+        store_pair(vrow, p, g, hd, dv[2 * p][kb], dv[2 * p + 1][kb]);
+      }
     }
   }
 }
