@@ -1255,16 +1255,21 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
       band[i] = v;
     }
     __syncthreads();
-    if (threadIdx.x < a.buckets) {
+    // a bucket's distances are shared out over the lanes of a group (at least two: 128 buckets, 256 threads)
+    int lanes = 64;
+    while (lanes * a.buckets > 256) lanes >>= 1;
+    const int u = threadIdx.x / lanes, first = threadIdx.x & (lanes - 1);
+    if (u < a.buckets) {
       int lo, hi;
-      bucket_range(a, tid, lo, hi);
+      bucket_range(a, u, lo, hi);
       float v = 0.f;
-      for (int i = lo; i <= hi; ++i) v += band[i + a.max_dist + kMargin];
-      if (lo == -a.max_dist - kMargin && lo <= hi)
+      for (int i = lo + first; i <= hi; i += lanes) v += band[i + a.max_dist + kMargin];
+      if (first == 0 && lo == -a.max_dist - kMargin && lo <= hi)
         for (int w = 0; w < 4 * GROUPS; ++w) v += fars[w * 2];
-      if (hi == a.right + kMargin && lo <= hi)
+      if (first == 0 && hi == a.right + kMargin && lo <= hi)
         for (int w = 0; w < 4 * GROUPS; ++w) v += fars[w * 2 + 1];
-      a.dtab[(((long long)b * nqt + qt) * a.nh + h) * a.buckets + tid] = v;
+      for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+      if (first == 0) a.dtab[(((long long)b * nqt + qt) * a.nh + h) * a.buckets + u] = v;
     }
   }
 }

@@ -128,18 +128,22 @@ __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, const T* __re
   float* all = reinterpret_cast<float*>(smem);
   for (int i = tid; i < size; i += 256) all[i] = (all[i] + all[size + i]) + (all[2 * size + i] + all[3 * size + i]);
   __syncthreads();
-  if (tid < a.buckets) {
-    // the distances of this bucket that lie strictly between the borders, then the far sums
+  // a bucket's distances that lie strictly between the borders, shared out over the lanes of a group, then the far sums
+  int lanes = 64;
+  while (lanes * a.buckets > 256) lanes >>= 1;
+  const int u = tid / lanes, part = tid & (lanes - 1);
+  if (u < a.buckets) {
     float v = 0.f;
     int lo, hi;
-    bucket_range(a, tid, lo, hi);
-    for (int d = max(lo, 1 - a.max_dist); d <= min(hi, a.right - 1); ++d) {
+    bucket_range(a, u, lo, hi);
+    for (int d = max(lo, 1 - a.max_dist) + part; d <= min(hi, a.right - 1); d += lanes) {
       const int i = d + a.max_dist;
       v += all[(i & 7) * eighth + (i >> 3)];
     }
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     if (lo <= -a.max_dist && hi >= -a.max_dist) v += far_l;
     if (hi >= a.right && lo <= a.right) v += far_r;
-    parts[((long long)blockIdx.x * a.heads + h) * a.buckets + tid] = v;
+    if (part == 0) parts[((long long)blockIdx.x * a.heads + h) * a.buckets + u] = v;
   }
 }
 
