@@ -68,17 +68,15 @@ template <> struct Frag<float> { f32x4 lo, hi; };
 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // Tile images in the LDS. bf16: rows of 64, 128 or 256 bytes (head sizes over 64 take 256) without padding, as the direct
-// loads need them, their 16-byte chunks permuted by an XOR with swz(row). With 64 banks of 4 bytes the 16 rows of a
-// ds_read_b128 fragment then fall on different banks, and so do the 8 rows of half a transposing read, whose lanes take
-// 32 bytes of each (two chunks whose indices differ in bit 0): the rows that share a bank offset get different swz for
-// the first and different swz >> 1 for the second. fp32: padded by 16 bytes, which spreads its 16- and 4-byte reads.
+// loads need them, their 16-byte chunks permuted by an XOR with swz(row). A ds_read_b128 serves 16 lanes at a time, lanes
+// 0-3, 12-15 and 20-27 (then 4-11, 16-19 and 28-31, then the same 32 up), a transposing read 32 lanes in order; with
+// these swizzles both fall on 64 different banks (counted: no conflict; with rows merely told apart 16 in order, the
+// fragment reads took twice their time). fp32: padded by 16 bytes, which spreads its 16- and 4-byte reads.
 template <typename T, int D> constexpr int row_stride() {
   return sizeof(T) == 4 ? D * 4 + 16 : (D == 32 ? 64 : D == 64 ? 128 : 256);
 }
 template <int STRIDE> __device__ __forceinline__ int swz(int row) {
-  if (STRIDE == 64) return ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
-  if (STRIDE == 128) return ((row >> 1) & 3) << 1 | ((row >> 3) & 1);
-  return (row & 7) << 1 | ((row >> 3) & 1);
+  return STRIDE == 64 ? (row >> 1) & 2 : STRIDE == 128 ? row & 6 : (row & 7) << 1;
 }
 
 __device__ __forceinline__ f32x4 mma(const Frag<unsigned short>& a, const Frag<unsigned short>& b, f32x4 c) {
