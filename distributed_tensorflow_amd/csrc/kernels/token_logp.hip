@@ -78,6 +78,13 @@ __device__ __forceinline__ u64 shfl_xor_u64(u64 v, int m) {
   return ((u64)hi << 32) | lo;
 }
 
+// the largest of three, a NaN if one of them is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 struct Shared {
   u64 cand[kCap];
   u64 best[kMaxTop];                 // the k best so far, descending
@@ -141,27 +148,32 @@ __global__ __launch_bounds__(NT, 6) void token_logp_fwd_kernel(const T* __restri
       in[u] = j < nvec;
       if (in[u]) r[u] = *reinterpret_cast<const u32x4_t*>(body + (long long)j * V);
     }
-    // running maximum, sum and sum of e^z z of this thread's elements
-    float cm = base == 0 ? xo : -INFINITY;
+    // running maximum, sum and sum of e^z z of this thread's elements; the maximum of each vector is kept for the search
+    const bool own = base == 0 && odd >= 0;
+    float vm[kU], cm = own ? xo : -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < kU; ++u) {
+      vm[u] = -INFINITY;
       if (in[u]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) cm = fmaxf(cm, Vec<T>::get(r[u], i));
+        for (int i = 0; i < V; i += 2) vm[u] = max3(vm[u], Vec<T>::get(r[u], i), Vec<T>::get(r[u], i + 1));
       }
-    const float mn = fmaxf(m, cm), ref = mn == -INFINITY ? 0.f : mn;
+    }
+#pragma unroll
+    for (int u = 0; u < kU; u += 2) cm = max3(cm, vm[u], vm[u + 1]);
+    const float mn = max3(m, m, cm), ref = mn == -INFINITY ? 0.f : mn;
     const float shift = m == -INFINITY ? kFloor : fmaxf(m - ref, kFloor), alpha = __builtin_amdgcn_exp2f(shift * kLog2e);
     w = alpha * fmaf(s, shift, w);
     s = alpha * s;
     m = mn;
     auto add = [&](float v) {
       float z = v - ref;
-      z = z < kFloor ? kFloor : z;                       // NaN stays NaN
+      z = max3(z, z, kFloor);
       const float e = __builtin_amdgcn_exp2f(z * kLog2e);
       s += e;
       w = fmaf(e, z, w);
     };
-    if (base == 0 && odd >= 0) add(xo);
+    if (own) add(xo);
 #pragma unroll
     for (int u = 0; u < kU; ++u)
       if (in[u]) {
@@ -170,31 +182,39 @@ __global__ __launch_bounds__(NT, 6) void token_logp_fwd_kernel(const T* __restri
       }
     if (!TOP) continue;
 
-    const bool some = in[0] || (base == 0 && odd >= 0);      // (chunks are filled from the front)
+    const bool some = in[0] || own;      // (chunks are filled from the front)
     if (base == 0) {
-      // first threshold: k-th largest of 64 maxima. The index in a thread's key is that of its first element where this
-      // is the maximum, otherwise its last one's: no element with the maximum has a lower key. An empty group has key 0
+      // first threshold: k-th largest of 64 maxima. The index in a thread's key is that of its first vector element where
+      // this is the maximum, otherwise C or more: no element with the maximum has a lower key. An empty group has key 0
       u64 key = 0ull;
-      if (some) {
-        const int first = in[0] ? head + tid * V : odd;
-        const float v0 = in[0] ? Vec<T>::get(r[0], 0) : xo;
-        key = key_of(cm, cm == v0 ? first : C + tid);
-      }
+      if (some) key = key_of(cm, in[0] && cm == Vec<T>::get(r[0], 0) ? head + tid * V : C + tid);
 #pragma unroll
       for (int o = 1; o < W; o <<= 1) {
         const u64 other = shfl_xor_u64(key, o);
         key = other > key ? other : key;
       }
-      if (lane % W == 0) sh.group[wid * (64 / W) + lane / W] = key;
-      __syncthreads();
+      if (W > 1) {
+        if (lane % W == 0) sh.group[wid * (64 / W) + lane / W] = key;
+        __syncthreads();
+      }
       if (wid == 0) {
-        const u64 mine = sh.group[lane];
-        int rank = 0;
-        for (int j = 0; j < 64; ++j) {
-          const u64 other = lane_u64(mine, j);
-          rank += other > mine || (other == mine && j < lane) ? 1 : 0;
-        }
-        if (rank == k - 1) sh.threshold = mine;
+        if (W > 1) key = sh.group[lane];
+        // the value bit by bit (a value of 16 bits has 16; below them a NaN's or a negative one's are all set). Where the
+        // last of the k is one of several equal groups, those of the lowest indexes are taken
+        constexpr unsigned kLow = sizeof(T) == 2 ? 0xffffu : 0u;
+        const unsigned value = (unsigned)(key >> 32) | kLow;
+        unsigned kth = kLow;
+#pragma unroll
+        for (unsigned bit = 0x80000000u; bit > kLow; bit >>= 1)
+          if (__popcll(__ballot(value >= (kth | bit))) >= k) kth |= bit;
+        const u64 equal = __ballot(value == kth);
+        const int need = k - __popcll(__ballot(value > kth));
+        const bool taken = value == kth && __popcll(equal & ((1ull << lane) - 1)) < need;
+        const bool vague = __ballot(taken && (unsigned)~(unsigned)key >= (unsigned)C) != 0ull;
+        // the lowest key of those taken: indexes ascend with the lane, but for the ones of C or more
+        const u64 lanes = __ballot(taken);
+        const u64 last = lane_u64(key, 63 - __builtin_clzll(lanes));
+        if (lane == 0) sh.threshold = vague ? last & ~0xffffffffull : last;
       }
       __syncthreads();
       threshold = sh.threshold;
@@ -202,30 +222,27 @@ __global__ __launch_bounds__(NT, 6) void token_logp_fwd_kernel(const T* __restri
     for (;;) {
       const float tv = value_of(threshold);
       // threshold 0: everything passes (value_of(0) is a NaN, which no element is below)
-      const bool scan = some && (!(cm < tv) || s != s);
       auto offer = [&](float v, int index) {
         const u64 key = key_of(v, index);
         if (key < threshold) return;
         const int at = atomicAdd(&sh.count, 1);
         if (at < kCap) sh.cand[at] = key;
       };
-      if (scan) {
-        if (base == 0 && odd >= 0 && !(xo < tv)) offer(xo, odd);
+      if (own && !(xo < tv)) offer(xo, odd);
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-          if (in[u]) {
-            // the elements are converted again, not kept in 32 registers from the sums above
-            asm volatile("" : "+v"(r[u]));
-            unsigned pass = 0;
+      for (int u = 0; u < kU; ++u)
+        if (in[u] && !(vm[u] < tv)) {
+          // the elements are converted again, not kept in 32 registers from the sums above
+          asm volatile("" : "+v"(r[u]));
+          unsigned pass = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) pass |= Vec<T>::get(r[u], i) < tv ? 0u : 1u << i;
-            while (pass) {
-              const int i = __builtin_ctz(pass);
-              pass &= pass - 1;
-              offer(Vec<T>::pick(r[u], i), head + (base + u * NT + tid) * V + i);
-            }
+          for (int i = 0; i < V; ++i) pass |= Vec<T>::get(r[u], i) < tv ? 0u : 1u << i;
+          while (pass) {
+            const int i = __builtin_ctz(pass);
+            pass &= pass - 1;
+            offer(Vec<T>::pick(r[u], i), head + (base + u * NT + tid) * V + i);
           }
-      }
+        }
       __syncthreads();
       const int count = sh.count;
       __syncthreads();                                   // (the next chunk counts on)
@@ -361,8 +378,13 @@ __global__ __launch_bounds__(NT) void token_logp_bwd_kernel(const T* __restrict_
   }
 }
 
-// 1024 threads a row where the rows are too few to fill the CUs, else 256 (less waiting at a barrier)
-bool wide_rows(int N, int C) { return C > 4096 && N < 512; }
+// Threads a row. One wave for short rows (nothing to wait for at a barrier; 64 / 256 threads, us, bf16, 5 alternatives:
+// 40000 x 4000 101 / 150, 20000 x 8000 85 / 89 and with 32 alternatives 143 / 120, 2048 x 131072 148 / 118), 1024
+// where long rows are too few to fill the CUs (256 x 131072, 256 / 1024 threads: 38 / 26)
+int fwd_threads(int N, int C) { return C <= 4096 ? 64 : N < 512 ? 1024 : 256; }
+// Backward (64 / 256 / 1024 threads, us: 80000 x 2000 144 / 167 / 476, 20000 x 8000 134 / 120 / 166, 12000 x 16000
+// 165 / 153 / 157, 5120 x 30522 143 / 136 / 127, 2048 x 131072 279 / 221 / 206: fewer rows at a time, written in longer runs)
+int bwd_threads(int N, int C) { return C <= 2048 ? 64 : C > 16384 || (C > 4096 && N < 512) ? 1024 : 256; }
 
 }  // namespace
 
@@ -373,12 +395,14 @@ DTF_API int dtf_token_logp_fwd(const void* x, const void* tokens, float* logp, f
                                int label_dtype, hipStream_t stream) {
   if (N <= 0) return 0;
   if (C <= 0 || ld < C || k < 0 || k > kMaxTop || k > C || N > kMaxRows || C > kMaxCols) return -1;
-  const bool wide = wide_rows(N, C);
+  const int nt = fwd_threads(N, C);
 #define FWD(T, L, NT, TOP)                                                                                            \
   hipLaunchKernelGGL((token_logp_fwd_kernel<T, L, NT, TOP>), dim3(N), dim3(NT), 0, stream, (const T*)x, (const L*)tokens, \
                      logp, entropy, top_logp, top_ids, stat, N, C, ld, k)
 #define FWD_L(T, L) \
-  if (wide) { if (k) FWD(T, L, 1024, true); else FWD(T, L, 1024, false); } else { if (k) FWD(T, L, 256, true); else FWD(T, L, 256, false); }
+  if (nt == 64) { if (k) FWD(T, L, 64, true); else FWD(T, L, 64, false); }        \
+  else if (nt == 256) { if (k) FWD(T, L, 256, true); else FWD(T, L, 256, false); } \
+  else { if (k) FWD(T, L, 1024, true); else FWD(T, L, 1024, false); }
   if (x_dtype == 0 && label_dtype == 0) { FWD_L(float, int) }
   else if (x_dtype == 0) { FWD_L(float, long long) }
   else if (label_dtype == 0) { FWD_L(unsigned short, int) }
@@ -396,11 +420,11 @@ DTF_API int dtf_token_logp_bwd(const void* x, const void* tokens, const float* s
   if (C <= 0 || ld < C || k < 0 || k > kMaxTop || k > C || N > kMaxRows || C > kMaxCols || (k && (!g_top || !top_ids)))
     return -1;
   if ((reinterpret_cast<uintptr_t>(x) & 15) != (reinterpret_cast<uintptr_t>(dx) & 15)) return -2;
-  const bool wide = wide_rows(N, C);
+  const int nt = bwd_threads(N, C);
 #define BWD(T, L, NT)                                                                                                  \
   hipLaunchKernelGGL((token_logp_bwd_kernel<T, L, NT>), dim3(N), dim3(NT), 0, stream, (const T*)x, (const L*)tokens, stat, \
                      entropy, top_ids, g_logp, g_ent, g_top, (T*)dx, N, C, ld, k)
-#define BWD_L(T, L) if (wide) BWD(T, L, 1024); else BWD(T, L, 256);
+#define BWD_L(T, L) if (nt == 64) BWD(T, L, 64); else if (nt == 256) BWD(T, L, 256); else BWD(T, L, 1024);
   if (x_dtype == 0 && label_dtype == 0) { BWD_L(float, int) }
   else if (x_dtype == 0) { BWD_L(float, long long) }
   else if (label_dtype == 0) { BWD_L(unsigned short, int) }

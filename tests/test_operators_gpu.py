@@ -325,6 +325,22 @@ def test_token_log_probs_of_degenerate_rows(dt, V):
     _compare_logp(x.to(dt), tok, 20, gs)
 
 
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N,V,top", [(600, 4097, 5), (513, 9001, 32), (2000, 1000, 20), (700, 300, 32)])
+def test_token_log_probs_of_many_rows(dt, N, V, top):
+    """As many rows as give each fewer threads; every seventh row is constant, every eleventh sorted, some masked to few."""
+    x, tok, g = _logits(N, V, dt)
+    x[::7] = 1.5
+    x[3::11] = (torch.arange(V) / V - 0.5).to(dt)
+    x[5::13, 40:] = -math.inf
+    x[6::13, : V - 9] = torch.finfo(dt).min
+    tok[9] = -1
+    tok[5::13] = 3
+    tok[6::13] = V - 1
+    gs = (torch.randn(N, generator=g), torch.randn(N, generator=g), torch.randn(N, top, generator=g))
+    _compare_logp(x, tok, top, gs)
+
+
 def test_token_log_probs_with_nan_and_infinity():
     from distributed_tensorflow_amd.ops.softmax_ce import token_log_probs
     x = torch.randn(3, 30000)
