@@ -105,6 +105,17 @@ __device__ __forceinline__ void pack(Frag<unsigned short>& f, const f32x4& a, co
   f.v = __builtin_bit_cast(bf16x8_t, r);
 }
 __device__ __forceinline__ void pack(Frag<float>& f, const f32x4& a, const f32x4& b) { f.lo = a; f.hi = b; }
+// what pack() rounded off
+__device__ __forceinline__ void pack_rest(Frag<unsigned short>& f, f32x4 a, f32x4 b, const Frag<unsigned short>& packed) {
+  const u32x4_t r = __builtin_bit_cast(u32x4_t, packed.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] -= __uint_as_float(i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
+    b[i] -= __uint_as_float(i & 1 ? r[2 + (i >> 1)] & 0xffff0000u : r[2 + (i >> 1)] << 16);
+  }
+  pack(f, a, b);
+}
+__device__ __forceinline__ void pack_rest(Frag<float>&, const f32x4&, const f32x4&, const Frag<float>&) {}
 
 // byte of a row's 16-byte chunk ch
 template <typename T, int D> __device__ __forceinline__ int chunk_at(int row, int ch) {
@@ -395,6 +406,9 @@ __device__ __forceinline__ void fill_band(const Args& a, int h, float* band, int
 }
 // What a kernel instance knows of the biases: none, the relative one alone, or a key bias with or without it.
 enum Mode { kPlain = 0, kRel = 1, kKeys = 2 };
+// Whether a forward pass may be asked for a table's gradient: then P enters O in two parts (see fwd_kernel).
+template <typename T, int MODE>
+constexpr bool two_parts() { return sizeof(T) == 2 && MODE != kPlain; }
 
 // the distances of bucket u, inclusive, clipped to the band
 __device__ __forceinline__ void bucket_range(const Args& a, int u, int& lo, int& hi) {
@@ -445,7 +459,11 @@ __device__ __forceinline__ void place(int pairs, int n, bool causal, int& pair, 
 }
 
 // ================================================================================================== forward
-template <typename T, int D, int MODE, int GROUPS>
+// PARTS 2: P enters O as two bf16 numbers, its rounding and what that left. D = rowsum(dO * O) takes over the roundings of the
+// P in O, each row's one error in all of its dT, and the sums over many rows in a table's gradient show it (relative error
+// against 64 bits 0.0015 to 0.0033 with one part, 0.0012 to 0.0018 with two, most of that dTable's own rounding; dQ and
+// dK, rounded more coarsely by themselves, keep theirs). 64 x 512 x 12 heads of 64: 91 us with one part, 111 with two.
+template <typename T, int D, int MODE, int GROUPS, int PARTS>
 __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) : (D <= 64 ? 2 : GROUPS))) void fwd_kernel(Args a) {
   constexpr int KT = key_tile<T>(), JB = KT / 16, DB = D / 16, DS = D / 32, IMG = Tile<T, D, KT>::IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V], [2][key bias of the tile], band
@@ -595,7 +613,6 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
           for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
         }
       }
-      Frag<T> pf[2][KT / 32];
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
         const float ref = m[qb] == -INFINITY ? 0.f : m[qb];          // nothing seen yet: every term is exp2(-inf)
@@ -609,18 +626,27 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
             sum += p;
           }
         l[qb] += sum;                                                // per lane; combined over the lane group at the end
-#pragma unroll
-        for (int ks = 0; ks < KT / 32; ++ks) pack(pf[qb][ks], s[2 * ks][qb], s[2 * ks + 1][qb]);
       }
 #pragma unroll
-      for (int ks = 0; ks < KT / 32; ++ks)
+      for (int ks = 0; ks < KT / 32; ++ks) {
+        Frag<T> pf[2], pr[2];
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          pack(pf[qb], s[2 * ks][qb], s[2 * ks + 1][qb]);
+          if (PARTS == 2) pack_rest(pr[qb], s[2 * ks][qb], s[2 * ks + 1][qb], pf[qb]);
+        }
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           Frag<T> vf;
           rd.read_tr(vf, vimg, db, ks);
 #pragma unroll
-          for (int qb = 0; qb < 2; ++qb) o[db][qb] = mma(vf, pf[qb][ks], o[db][qb]);
+          for (int qb = 0; qb < 2; ++qb) o[db][qb] = mma(vf, pf[qb], o[db][qb]);
+          if (PARTS == 2) {
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) o[db][qb] = mma(vf, pr[qb], o[db][qb]);
+          }
         }
+      }
     }
     if (t + GROUPS < nt) put(t + GROUPS);
     __syncthreads();
@@ -723,6 +749,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
   const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
   const bool rel = MODE == kRel || (MODE == kKeys && a.table);
+  const bool two = two_parts<T, MODE>() && a.table && a.fine;      // see fwd_kernel's PARTS
 
   if (rel) {
     for (int i = tid; i < group * a.buckets; i += 256) {
@@ -825,7 +852,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
       *reinterpret_cast<u32x4_t*>(vimg + chunk_at<T, D>(row, ch)) = vr[u];
     }
     if (t + 4 < t1) fetch(t + 4);
-    Frag<T> pf[QB];
+    Frag<T> pf[QB], pr[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const int end = a.causal ? min(klen, pos[qb] + 1) : klen;
@@ -852,6 +879,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db][qb] *= alpha;
       pack(pf[qb], s[0][qb], s[1][qb]);
+      if (two) pack_rest(pr[qb], s[0][qb], s[1][qb], pf[qb]);
     }
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -859,7 +887,10 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
       Frag<T> vf;
       rd.read_tr(vf, vimg, db, 0);
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) o[db][qb] = mma(vf, pf[qb], o[db][qb]);
+      for (int qb = 0; qb < QB; ++qb) {
+        o[db][qb] = mma(vf, pf[qb], o[db][qb]);
+        if (two) o[db][qb] = mma(vf, pr[qb], o[db][qb]);
+      }
     }
     asm volatile("" ::: "memory");
   }
@@ -1554,17 +1585,20 @@ inline int dkdv_splits(int B, int Sk, int nh, int nkv) {
 // too few waves to hide a tile's chain of products and exponentials, and for sequences long enough to share out.
 inline bool two_groups(long long blocks, int tiles, int D) { return blocks <= (D <= 64 ? 1024 : 256) && tiles >= 4; }
 
-template <typename T, int D, int MODE, int GROUPS>
+template <typename T, int D, int MODE, int GROUPS, int PARTS>
 int run_fwd_as(const Args& a, long long n, hipStream_t stream) {
   const int lds = GROUPS * (lds_tiles<T, D>() + 8 * key_tile<T>()) + 4 * (GROUPS > 1 && band_floats(a) < 1024 ? 1024 : band_floats(a));
-  return launch(fwd_kernel<T, D, MODE, GROUPS>, n, 256 * GROUPS, lds, a, stream);
+  return launch(fwd_kernel<T, D, MODE, GROUPS, PARTS>, n, 256 * GROUPS, lds, a, stream);
 }
 template <typename T, int D, int MODE>
 int run_fwd(const Args& a, hipStream_t stream) {
   if (few_queries(a.Sq, a.nh, a.nkv))
     return a.Sq * (a.nh / a.nkv) <= 16 ? run_few<T, D, 1, MODE>(a, stream) : run_few<T, D, 2, MODE>(a, stream);
   const long long n = (long long)a.B * a.nh * ((a.Sq + kRows - 1) / kRows);
-  return two_groups(n, a.Sk / key_tile<T>(), D) ? run_fwd_as<T, D, MODE, 2>(a, n, stream) : run_fwd_as<T, D, MODE, 1>(a, n, stream);
+  const bool two = two_groups(n, a.Sk / key_tile<T>(), D);
+  if constexpr (two_parts<T, MODE>())
+    if (a.table && a.fine) return two ? run_fwd_as<T, D, MODE, 2, 2>(a, n, stream) : run_fwd_as<T, D, MODE, 1, 2>(a, n, stream);
+  return two ? run_fwd_as<T, D, MODE, 2, 1>(a, n, stream) : run_fwd_as<T, D, MODE, 1, 1>(a, n, stream);
 }
 template <typename T, int D, int MODE, int GROUPS>
 int run_dq(const Args& a, long long n, hipStream_t stream) {
@@ -1614,12 +1648,24 @@ int run_f32_keys(const Args& a, bool backward, hipStream_t s);
 
 // The kernels of one (type, mode), named one by one: left to the launches in by_head_size, the host pass drops some.
 #define DTF_ATTN_KERNELS(T, D, M)                            \
-  template __global__ void fwd_kernel<T, D, M, 1>(Args);      \
-  template __global__ void fwd_kernel<T, D, M, 2>(Args);      \
+  template __global__ void fwd_kernel<T, D, M, 1, 1>(Args);   \
+  template __global__ void fwd_kernel<T, D, M, 2, 1>(Args);   \
   template __global__ void bwd_dq_kernel<T, D, M, 1>(Args);   \
   template __global__ void bwd_dq_kernel<T, D, M, 2>(Args);   \
   template __global__ void bwd_dkdv_kernel<T, D, M, 1>(Args); \
   template __global__ void bwd_dkdv_kernel<T, D, M, 2>(Args);
+#define DTF_ATTN_KERNELS_2(D, M)                                         \
+  template __global__ void fwd_kernel<unsigned short, D, M, 1, 2>(Args); \
+  template __global__ void fwd_kernel<unsigned short, D, M, 2, 2>(Args);
+#define DTF_ATTN_TWO_PARTS(M)  \
+  namespace dtf {              \
+  namespace attn {             \
+  DTF_ATTN_KERNELS_2(32, M)    \
+  DTF_ATTN_KERNELS_2(64, M)    \
+  DTF_ATTN_KERNELS_2(96, M)    \
+  DTF_ATTN_KERNELS_2(128, M)   \
+  }                            \
+  }
 #define DTF_ATTN_INSTANCE(NAME, T, M)                                                   \
   namespace dtf {                                                                       \
   namespace attn {                                                                      \

@@ -234,6 +234,36 @@ def test_attention_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(outs, new)), i
 
 
+@pytest.mark.parametrize("Sq,masked", [(40, False), (40, True), (7, False)], ids=["rows", "key_bias", "few"])
+def test_table_gradient_of_bf16_attention_is_finer_than_bf16(Sq, masked):
+    """An fp32 table beside bf16 q, k, v. Nothing that a row's dT = P (dP - D) is made of may be rounded to 8 bits: P enters
+    O in two parts of 8 bits and D reads O to 16. Bound: D off by 2^-17 of sum P |dP| and of sum |dO O| each, doubled; P and
+    dP by fp32 roundings, 64 + 64 terms of 2^-24 and an exponent of up to 16, below 2^-17."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    Sk, nh, hd, buckets = 90, 3, 64, 8
+    q, k, v, do, table = _inputs(1, Sq, Sk, nh, nh, hd, BF16, buckets)
+    table = 0.5 * table.float()
+    bias = torch.where(torch.arange(Sk) % 9 == 0, -1.0, 0.0)[None] if masked else None
+    d = torch.arange(Sk)[None, :] - (torch.arange(Sq)[:, None] + Sk - Sq)
+    of = O.buckets_between(int(d.min()), int(d.max()), buckets, 30, True)[d - int(d.min())]
+    want, tol = torch.zeros(buckets, nh, dtype=torch.float64), torch.zeros(buckets, nh, dtype=torch.float64)
+    for h in range(nh):
+        qq, kk, vv, dd = (t[0, :, h].double() for t in (q, k, v, do))
+        t = qq @ kk.t() / math.sqrt(hd) + table[:, h].double()[of] + (bias.double() if masked else 0.0)
+        p = torch.softmax(t, 1)
+        dp, o = dd @ vv.t(), p @ vv
+        D = (dd * o).sum(1, keepdim=True)
+        off = 2.0 ** -16 * ((p * dp.abs()).sum(1, keepdim=True) + (dd * o).abs().sum(1, keepdim=True))
+        mag = dd.abs() @ vv.abs().t() + D.abs()
+        for u in range(buckets):
+            want[u, h] = (p * (dp - D))[of == u].sum()
+            tol[u, h] = (p * (off + 2.0 ** -17 * mag))[of == u].sum() + 1e-30       # (0 in a bucket with no distance)
+    leaf = table.to(DEV).requires_grad_()
+    out = attention(q.to(DEV), k.to(DEV), v.to(DEV), _dev(bias), rel_table=leaf, rel_max_distance=30)
+    got, = torch.autograd.grad(out, leaf, do.to(DEV))
+    O.check("dtable", got, want, tol)
+
+
 # ------------------------------------------------------------------------------------------------ relative bias
 @pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("cfg", [(1, 1, 3, 32, 128, True), (70, 70, 2, 32, 128, True), (129, 300, 3, 16, 50, False),
