@@ -17,7 +17,24 @@ The reference has no counterpart: it runs TensorFlow eagerly, one op at a time
 """
 from __future__ import annotations
 
+import contextlib
+import gc
+
 import torch
+
+
+@contextlib.contextmanager
+def collected():
+    """For a capture: Python's garbage is collected before it and not during it. A graph that died in a reference cycle (a
+    step callable and what holds it, say) may not be freed while another one is captured: that ends the process."""
+    gc.collect()
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if was:
+            gc.enable()
 
 
 def _sig(t):
@@ -88,7 +105,7 @@ class GraphedStep:
         sx, sy = _clone_static(x), _clone_static(y)
         torch.cuda.synchronize(self.device)
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g, pool=self._pool):
+        with collected(), torch.cuda.graph(g, pool=self._pool):
             loss = self.step_fn(sx, sy)
         if self._pool is None:
             self._pool = g.pool()
