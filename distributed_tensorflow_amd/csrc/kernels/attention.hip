@@ -113,7 +113,7 @@ DTF_API int dtf_attention_bwd_splits(int B, int Sk, int nh, int nkv) { return nk
 // Key splits of the forward pass. More than one: it needs a scratch of splits * B * nh * Sq * (hd rounded up to 32, + 2)
 // floats.
 DTF_API int dtf_attention_splits(int B, int Sq, int Sk, int nh, int nkv) {
-  return nkv > 0 && attn::few_queries(Sq, nh, nkv) ? attn::few_splits(B, Sk, nkv) : 1;
+  return B > 0 && nkv > 0 && attn::few_queries(Sq, nh, nkv) ? attn::few_splits(B, Sk, nkv) : 1;
 }
 
 DTF_API int dtf_attention_fwd(const long long* words, int n_words, float scale, hipStream_t stream) {

@@ -207,19 +207,23 @@ def _dense(p, S, n, hd):
     return p, S * n * hd, n * hd, hd
 
 
+def _inputs(q, k, v, nkv):
+    """q, k, v as the kernels read them, and their twelve words."""
+    q, w = _usable(q)
+    if k is None:
+        return q, k, v, _heads(q, w, q.shape[2] - 2 * nkv, nkv)
+    (k, kw), (v, vw) = _usable(k), _usable(v)
+    return q, k, v, (*w, *kw, *vw)
+
+
 def _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat, fine):
     """(out, q, k, v as the kernels read them, table, words of the call)."""
     causal, scale, start0, max_distance, bidirectional = opts
-    q, qw = _usable(q)
+    q, k, v, ins = _inputs(q, k, v, nkv)
     B, Sq, nh, hd = q.shape
     if k is None:
         nh -= 2 * nkv
-        Sk = Sq
-        ins = _heads(q, qw, nh, nkv)
-    else:
-        (k, kw), (v, vw) = _usable(k), _usable(v)
-        Sk = k.shape[1]
-        ins = (*qw, *kw, *vw)
+    Sk = Sq if k is None else k.shape[1]
     out = torch.empty(B, Sq, nh, hd, dtype=q.dtype, device=q.device)
     bf16, rel, borders = int(q.dtype == torch.bfloat16), (0, 0, 0), ()
     if table is not None:
@@ -227,7 +231,7 @@ def _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat, fine):
         rel = (table.data_ptr(), int(table.dtype == torch.bfloat16), table.shape[0])
         borders = _rel.bucket_borders(table.shape[0], max_distance, bidirectional)
     part, splits = 0, 1
-    if Sq * nh <= 32 * nkv and Sk > 256:           # few queries: the keys may be split over workgroups
+    if B and Sq * nh <= 32 * nkv and Sk > 256:           # few queries: the keys may be split over workgroups
         splits = _lib.kernels().dtf_attention_splits(B, Sq, Sk, nh, nkv)
         if splits > 1:
             part = torch.empty(splits * B * nh * Sq * (-(-hd // 32) * 32 + 2), dtype=torch.float32, device=q.device)
@@ -257,16 +261,19 @@ class _GeneralFn(torch.autograd.Function):
             fine = torch.empty(B, Sq, n - 2 * nkv if k is None else n, q.shape[3], dtype=torch.uint8, device=q.device)
         out, q, k, v, table, ctx.words = _forward(q, k, v, table, key_bias, lens, starts, nkv, opts, stat, fine)
         ctx.scale = opts[1]
-        # (the words point into these)
         ctx.save_for_backward(q, k, v, table, key_bias, lens, starts, stat, fine, out)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, *_, out = ctx.saved_tensors
-        words, dev, dt = ctx.words, q.device, q.dtype
+        # the words of the forward pass hold the sizes; what they point to may have moved (hooks on saved tensors put them
+        # elsewhere, checkpointing computes them anew)
+        q, k, v, table, key_bias, lens, starts, stat, fine, out = ctx.saved_tensors
+        words = ctx.words
         B, Sq, Sk, nh, nkv, hd = words[45:51]
+        q, k, v, ins = _inputs(q, k, v, nkv)
+        dev, dt = q.device, q.dtype
         dq = torch.empty(q.shape, dtype=dt, device=dev)
         dk = dv = dtable = None
         if k is None:
@@ -292,8 +299,10 @@ class _GeneralFn(torch.autograd.Function):
             if splits > 1:
                 part = torch.empty(splits * 2 * B * nkv * Sk * (-(-hd // 32) * 32), dtype=torch.float32, device=dev)
         dout, dw = _usable(dout)
-        _call("dtf_attention_bwd", (*words[:16], *dw, *grads, *words[32:42], p, *((0, 0) if dtable is None else
-              (p + 4 * n, dtable.data_ptr())), *words[45:53], part.data_ptr() if splits > 1 else 0, *words[54:]), ctx.scale, q)
+        keys, lengths, first, bias, stats, low = (0 if t is None else t.data_ptr() for t in (key_bias, lens, starts, table, stat, fine))
+        _call("dtf_attention_bwd", (*ins, *_dense(out.data_ptr(), Sq, nh, hd), *dw, *grads, keys, lengths, first, words[35], bias,
+              *words[37:41], stats, p, *((0, 0) if dtable is None else (p + 4 * n, dtable.data_ptr())), *words[45:53],
+              part.data_ptr() if splits > 1 else 0, low, *words[55:]), ctx.scale, q)
         return dq, dk, dv, dtable, None, None, None, None, None
 
 
@@ -330,7 +339,9 @@ def _composed(q, k, v, table, key_bias, lens, starts, nkv, opts):
 def _int_vector(t, name, B, device):
     if not isinstance(t, torch.Tensor) or t.shape != (B,) or t.dtype not in (torch.int32, torch.int64) or t.device != device:
         raise ValueError(f"{name} is an int32 or int64 tensor [{B}] on {device}")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:                     # (values that 32 bits do not hold stay as far out as they are)
+        t = t.clamp(-(1 << 30), 1 << 30).int()
+    return t.contiguous()
 
 
 def _general(q, k, v, nkv, key_bias, causal, scale, key_lengths, q_start, rel_table, rel_max_distance, rel_bidirectional):
@@ -341,7 +352,7 @@ def _general(q, k, v, nkv, key_bias, causal, scale, key_lengths, q_start, rel_ta
         raise ValueError(f"head size {hd}: need a multiple of 8 up to 128")
     if nkv < 1 or nh < 1 or nh % nkv:
         raise ValueError(f"{nh} query heads do not divide over {nkv} key / value heads")
-    if max(B, Sq, Sk) > 1 << 28 or nh > 1 << 16:
+    if max(B, Sq, Sk) > 1 << 28 or nh > 1 << 16 or n * hd > 1 << 22:
         raise ValueError(f"sizes {tuple(q.shape)} with {Sk} keys are out of range")
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     if not 1e-30 < scale < 1e30:

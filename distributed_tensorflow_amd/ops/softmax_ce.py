@@ -174,6 +174,8 @@ class _TokenLogp(torch.autograd.Function):
         x, y, stat, entropy, top_ids = ctx.saved_tensors
         if g_logp is None and g_ent is None and g_top is None:
             return None, None, None
+        if not _row_padded(x):                     # (hooks on saved tensors may lay it out anew)
+            x = x.contiguous()
         g_logp, g_ent, g_top = (None if g is None else g.float().contiguous() for g in (g_logp, g_ent, g_top))
         N, C = x.shape
         ld = x.stride(0) if N > 1 else C

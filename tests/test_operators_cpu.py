@@ -44,6 +44,21 @@ def test_attention_refuses(kw, err):
         attention(args.pop("q"), args.pop("k"), args.pop("v"), **args)
 
 
+def test_attention_refuses_rows_wider_than_its_offsets():
+    x = torch.empty(1, 1, 65536, 72)
+    with pytest.raises(ValueError):
+        attention(x, x, x)
+    with pytest.raises(ValueError):
+        self_attention(x, kv_heads=16384)
+
+
+def test_splits_of_an_empty_batch():
+    from distributed_tensorflow_amd.ops import _lib
+    lib = _lib.kernels()
+    assert lib.dtf_attention_splits(0, 1, 4001, 16, 4) == 1 and lib.dtf_attention_splits(8, 1, 4001, 16, 4) > 1
+    assert lib.dtf_attention_bwd_splits(0, 4001, 16, 4) >= 1
+
+
 def test_self_attention_refuses():
     for x, kw in ((_t(2, 5, 8, 16), dict(kv_heads=4)), (_t(2, 5, 8, 16), dict(kv_heads=0)), (_t(2, 5, 7, 16), dict(kv_heads=2)),
                   (_t(2, 5, 2, 4, 16), dict(causal=True)), (_t(2, 5, 3, 4, 16), dict(kv_heads=4)), (_t(2, 5, 8, 16), dict(causal=True))):
@@ -138,3 +153,25 @@ def test_token_log_probs_torch_form():
     rows = torch.tensor([0, 1, 2, 3])                     # (rows with infinities: the kernels' business)
     d, = torch.autograd.grad((r.logp[rows], r.entropy[rows], r.top_logp[rows]), leaf, [g[rows] for g in gs])
     O.check("dlogits", d[rows], val["dlogits"][rows], tol["dlogits"][rows])
+
+
+def test_no_garbage_is_collected_while_a_graph_is_captured():
+    import gc
+    import weakref
+    from distributed_tensorflow_amd.engine.graph import collected
+
+    class Node:
+        pass
+
+    def cycle():
+        a = Node()
+        a.me = a
+        return weakref.ref(a)
+
+    old = cycle()
+    with collected():
+        assert old() is None and not gc.isenabled()
+        new = cycle()
+        kept = [[] for _ in range(20000)]                # (more than one generation's worth of containers)
+        assert new() is not None and kept
+    assert gc.isenabled()

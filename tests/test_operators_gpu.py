@@ -9,6 +9,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(__file__))
 import operator_oracles as O  # noqa: E402
+from distributed_tensorflow_amd.engine.graph import collected  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -223,7 +224,7 @@ def test_attention_on_another_stream_and_in_a_graph():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     del got
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with collected(), torch.cuda.graph(g):
         outs = run(leaves)
     for i in range(4):
         with torch.no_grad():
@@ -262,6 +263,58 @@ def test_table_gradient_of_bf16_attention_is_finer_than_bf16(Sq, masked):
     out = attention(q.to(DEV), k.to(DEV), v.to(DEV), _dev(bias), rel_table=leaf, rel_max_distance=30)
     got, = torch.autograd.grad(out, leaf, do.to(DEV))
     O.check("dtable", got, want, tol)
+
+
+@pytest.mark.parametrize("how", ["offload", "checkpoint"])
+def test_gradients_with_saved_tensors_moved(how):
+    """Hooks put what the backward pass needs elsewhere (the forward's own copies are freed), or it is computed anew."""
+    from torch.utils.checkpoint import checkpoint
+    from distributed_tensorflow_amd.ops.attention import attention, self_attention
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    from distributed_tensorflow_amd.ops.softmax_ce import token_log_probs
+    q, k, v, do, table = (t.to(DEV) for t in _inputs(2, 130, 130, 4, 2, 64, BF16, 32))
+    bias = torch.zeros(2, 130, device=DEV)
+    bias[0, 100:] = -math.inf
+    lens = torch.tensor([130, 90], device=DEV)
+    tok = torch.arange(260, device=DEV)
+
+    def step(q, k, v, table):
+        wide = torch.cat((q, k, v), 2) * 1.5                       # (only the graph holds these)
+        a = attention(q * 2, k * 2, v * 2, bias * 1, rel_table=table * 2, causal=True)
+        b = self_attention(wide, kv_heads=2, key_lengths=lens + 0, rel_table=table * 3)
+        r = token_log_probs((a + b).reshape(260, 256)[:, :250] * 1, tok, 3)
+        w = relative_bias(table * 2, 130, 130)
+        return (a * do).float().sum() + (b * do).float().sum() + r.logp.sum() + r.top_logp.sum() + r.entropy.sum() + w.float().sum()
+
+    def grads(run):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+        loss = run(leaves)
+        junk = [torch.full((1 << n,), math.nan, device=DEV) for n in range(8, 22)]       # over whatever was freed
+        return torch.autograd.grad(loss, leaves), junk
+
+    def moved(leaves):
+        if how == "checkpoint":
+            return checkpoint(step, *leaves, use_reentrant=False)
+        with torch.autograd.graph.save_on_cpu():
+            return step(*leaves)
+
+    want, got = grads(lambda leaves: step(*leaves))[0], grads(moved)[0]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_attention_of_no_sequences_and_of_lengths_beyond_32_bits():
+    from distributed_tensorflow_amd.ops.attention import attention
+    for B, Sq in ((0, 1), (0, 200), (2, 0)):
+        q, k, v, do, _ = (None if t is None else t.to(DEV) for t in _inputs(B, Sq, 400, 4, 2, 64, BF16))
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        out = attention(*leaves, causal=True)
+        assert out.shape == (B, Sq, 4, 64)
+        assert all(float(g.abs().sum()) == 0 for g in torch.autograd.grad(out, leaves, do))
+        assert attention(q.detach(), k.detach(), v.detach()).shape == out.shape
+    q, k, v, _, _ = (None if t is None else t.to(DEV) for t in _inputs(3, 70, 90, 2, 2, 64, FP32))
+    far = torch.tensor([1 << 40, -(1 << 33), (1 << 32) + 5], device=DEV)
+    assert torch.equal(attention(q, k, v, key_lengths=far), attention(q, k, v, key_lengths=far.clamp(0, 90).int()))
+    assert torch.equal(attention(q, k, v, q_start=far, causal=True), attention(q, k, v, q_start=far.clamp(-200, 200), causal=True))
 
 
 # ------------------------------------------------------------------------------------------------ relative bias
@@ -431,7 +484,7 @@ def test_token_log_probs_in_a_graph():
         run(leaf)
     torch.cuda.current_stream().wait_stream(side)
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with collected(), torch.cuda.graph(g):
         outs = run(leaf)
     for i in range(4):
         with torch.no_grad():
@@ -560,7 +613,7 @@ def test_operators_in_two_graphs_and_on_two_streams_at_once():
     graphs, outs = [], []
     for r in runs:
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with collected(), torch.cuda.graph(g):
             outs.append(r())
         graphs.append(g)
     for _ in range(3):
