@@ -265,6 +265,24 @@ def test_table_gradient_of_bf16_attention_is_finer_than_bf16(Sq, masked):
     O.check("dtable", got, want, tol)
 
 
+def test_attention_over_a_cache_that_passes_32_bits():
+    """Rows 2^22 elements apart (the widest that are read in place): the last ones lie 5 GB behind the first."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    Sk, row = 650, 1 << 22
+    buf = torch.empty(Sk * row, dtype=BF16, device=DEV)
+    kv = buf.as_strided((1, Sk, 4, 64), (Sk * row, row, 64, 1))
+    kv.copy_(torch.randn(1, Sk, 4, 64, generator=torch.Generator().manual_seed(3)).to(BF16))
+    for Sq in (1, 70):
+        q, _, _, do, _ = (None if t is None else t.to(DEV) for t in _inputs(1, Sq, Sk, 4, 2, 64, BF16))
+
+        def run(kv):
+            leaves = [t.requires_grad_() for t in (q.clone(), kv[:, :, :2].detach(), kv[:, :, 2:].detach())]
+            out = attention(*leaves, causal=True)
+            return [out, *torch.autograd.grad(out, leaves, do)]
+
+        assert all(torch.equal(a, b) for a, b in zip(run(kv), run(kv.contiguous())))
+
+
 @pytest.mark.parametrize("how", ["offload", "checkpoint"])
 def test_gradients_with_saved_tensors_moved(how):
     """Hooks put what the backward pass needs elsewhere (the forward's own copies are freed), or it is computed anew."""
