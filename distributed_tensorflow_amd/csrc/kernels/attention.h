@@ -1556,7 +1556,8 @@ inline int launch(K kernel, long long blocks, int threads, int lds, const Args& 
 }
 
 // Key splits of the few-queries path: two workgroups a CU, and at least two key tiles for each of a workgroup's waves
-// (fewer and the joining costs more than the splitting gains). 1: no second kernel.
+// (fewer and the joining costs more than the splitting gains; 8 sequences x 4001 keys, 16 heads on 4 of 128: 12 + 4 us
+// against 100 unsplit). 1: no second kernel.
 inline bool few_queries(int Sq, int nh, int nkv) { return (long long)Sq * (nh / nkv) <= kFewRows; }
 inline int few_splits(int B, int Sk, int nkv) {
   const long long groups = (long long)B * nkv, most = (Sk + 8 * kFewKeys - 1) / (8 * kFewKeys);
@@ -1573,7 +1574,8 @@ int run_few(const Args& a, hipStream_t stream) {
   hipLaunchKernelGGL((few_join_kernel<T, D, MODE>), dim3((unsigned)(a.B * a.nh * a.Sq)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
-// Splits of the dK / dV kernel over the query heads of a key head, so that about three workgroups come to a CU.
+// Splits of the dK / dV kernel over the query heads of a key head, so that about three workgroups come to a CU (4 x 2048
+// causal, 16 heads on 4 of 128, with the joining: 4 splits 180 + 24 us, 2 splits 225 + 14).
 inline int dkdv_splits(int B, int Sk, int nh, int nkv) {
   const long long n = (long long)B * nkv * ((Sk + kRows - 1) / kRows), group = nh / nkv;
   for (long long s = 1; s < group; ++s)
@@ -1581,9 +1583,18 @@ inline int dkdv_splits(int B, int Sk, int nh, int nkv) {
   return (int)group;
 }
 
-// Workgroups of eight waves instead of four, whose two halves walk every other tile: for grids that leave the CUs with
-// too few waves to hide a tile's chain of products and exponentials, and for sequences long enough to share out.
-inline bool two_groups(long long blocks, int tiles, int D) { return blocks <= (D <= 64 ? 1024 : 256) && tiles >= 4; }
+// Workgroups of eight waves instead of four, whose two halves walk every other tile: for grids that leave the CUs with too
+// few waves to hide a tile's chain of products and exponentials. Otherwise the smaller ones fill the CUs better. Kernel
+// times in us, one / two halves, forward, dQ, dK / dV, heads of 64 if not said:
+//   at most a workgroup a CU: 4 x 512 x 12 heads 13.6 / 13.1, 15.7 / 15.4, 17.4 / 14.4; 2048 x 16 of 128 52 / 44, 67 / 56,
+//     111 / 100; more of them: 10 x 512 x 12 18 / 19, 21 / 28, 25 / 27, 16 x 512 x 12 26 / 28, 31 / 43, 35 / 44, 8 x 1000 keys
+//     x 10 of 80 (640 workgroups) dK / dV 39 / 47, 4 x 2048 causal x 16 of 128 94 / 103, 126 / 144, 184 / 248
+//   long rows, heads up to 64: 4096 x 16 95 / 86, 101 / 106, 133 / 134, causal 8192 x 8 148 / 113, 151 / 148, 199 / 187,
+//     x 12 209 / 181, 213 / 201, 279 / 255, 2 x 8192 x 8 215 / 198, 218 / 249, 281 / 317
+inline bool two_groups(long long blocks, int tiles, int D, bool backward, bool causal) {
+  if (tiles < 4 || blocks <= 256) return tiles >= 4;
+  return D <= 64 && tiles >= 32 && (backward ? causal && blocks <= 768 : blocks <= 1024);
+}
 
 template <typename T, int D, int MODE, int GROUPS, int PARTS>
 int run_fwd_as(const Args& a, long long n, hipStream_t stream) {
@@ -1595,7 +1606,7 @@ int run_fwd(const Args& a, hipStream_t stream) {
   if (few_queries(a.Sq, a.nh, a.nkv))
     return a.Sq * (a.nh / a.nkv) <= 16 ? run_few<T, D, 1, MODE>(a, stream) : run_few<T, D, 2, MODE>(a, stream);
   const long long n = (long long)a.B * a.nh * ((a.Sq + kRows - 1) / kRows);
-  const bool two = two_groups(n, a.Sk / key_tile<T>(), D);
+  const bool two = two_groups(n, a.Sk / key_tile<T>(), D, false, a.causal);
   if constexpr (two_parts<T, MODE>())
     if (a.table && a.fine) return two ? run_fwd_as<T, D, MODE, 2, 2>(a, n, stream) : run_fwd_as<T, D, MODE, 1, 2>(a, n, stream);
   return two ? run_fwd_as<T, D, MODE, 2, 1>(a, n, stream) : run_fwd_as<T, D, MODE, 1, 1>(a, n, stream);
@@ -1618,9 +1629,9 @@ int run_bwd(const Args& a, hipStream_t stream) {
   const long long nq = (long long)a.B * a.nh * nqt, nk = (long long)a.B * a.nkv * nkt * a.ksplits;
   // (a long band of sums for each of eight waves may not fit)
   const bool fits = 2 * (lds_tiles<T, D>() + 8 * kt) + 4 * (9 * band_floats(a) + 16) <= kMaxLds;
-  int rc = two_groups(nq, a.Sk / kt, D) && fits ? run_dq<T, D, MODE, 2>(a, nq, stream) : run_dq<T, D, MODE, 1>(a, nq, stream);
+  int rc = two_groups(nq, a.Sk / kt, D, true, a.causal) && fits ? run_dq<T, D, MODE, 2>(a, nq, stream) : run_dq<T, D, MODE, 1>(a, nq, stream);
   if (rc) return rc;
-  rc = two_groups(nk, a.Sq / kt, D) ? run_dkdv<T, D, MODE, 2>(a, nk, stream) : run_dkdv<T, D, MODE, 1>(a, nk, stream);
+  rc = two_groups(nk, a.Sq / kt, D, true, a.causal) ? run_dkdv<T, D, MODE, 2>(a, nk, stream) : run_dkdv<T, D, MODE, 1>(a, nk, stream);
   if (rc || a.ksplits == 1) return rc;
   const long long n = (long long)a.B * a.nkv * a.Sk * (D / 4);
   hipLaunchKernelGGL((dkdv_join_kernel<T, D>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
