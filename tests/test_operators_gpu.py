@@ -358,6 +358,20 @@ def test_relative_bias(dt, cfg, q_start):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("q_len,k_len", [(4003, 5001), (2999, 7003)])
+def test_relative_bias_larger_than_the_caches(dt, q_len, k_len):
+    """Every row at another alignment, most of it beyond the band: the values of the table at the oracle's buckets."""
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    heads, buckets = 11, 32
+    table = torch.randn(buckets, heads, generator=torch.Generator().manual_seed(5)).to(dt).to(DEV)
+    bias = relative_bias(table, q_len, k_len, q_start=700)
+    low = -(q_len - 1) - 700
+    of = O.buckets_between(low, k_len - 1 - 700, buckets, 128, True).to(DEV)
+    for h in range(heads):
+        assert torch.equal(bias[h], table[:, h][of].unfold(0, k_len, 1).flip(0)), h
+
+
 def test_attention_adds_the_bias_that_relative_bias_writes():
     """Both entry points read a table the same way: key biases made of its rows for one query."""
     from distributed_tensorflow_amd.ops.attention import attention
