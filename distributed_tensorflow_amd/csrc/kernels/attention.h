@@ -15,6 +15,13 @@
 //
 // Scores are kept in units of 1 / (scale log2 e): the biases are divided by that factor where they are staged and enter
 // as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score.
+//
+// Measured (bf16, us and the rate of the products): 64 x 512 tokens x 12 heads of 64, with a table: forward 111 (P in two
+// parts, see PARTS), dQ and dTable 174, dK / dV 157; without one 85, 111, 133 (610, 695, 775 TFLOP/s of what each has to do);
+// 4 x 8192 x 12 of 64, not causal: 955, 1243, 1265 TFLOP/s; 4 x 2048 causal, 16 heads on 4 of 128: 94, 125, 183 and 24 for
+// the join. Long rows are bound by the vector instructions beside the products (the forward pass keeps them 70 % busy:
+// maximum, exponential, sum, conversion of every score); at 512 tokens and less by a workgroup's beginning and end, where
+// it waits for memory.
 #pragma once
 #include "dtf_common.h"
 
@@ -977,7 +984,7 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a) {
 // exactly the place of the NEXT block's rotation: selecting between e_J and e_(J-1) before the rotation makes every lane
 // right. Three such rotations fold r away, then one by 4 g per lane group folds g, and two half swaps sum the lane groups
 // and put two blocks side by side: 32 lanes with 32 consecutive distances, one LDS addition per 32 x 32 scores where one
-// per register with colliding lanes (ds_add_f32, 12 of them) took three quarters of the kernel (0.54 ms instead of 0.16 at
+// per register with colliding lanes (ds_add_f32, 12 of them) took three quarters of the kernel (0.54 ms instead of 0.17 at
 // 64 x 512 tokens, 12 heads of 64). Every sum has a fixed order.
 struct DiagonalSums {
   f32x4 carry, prev;                 // block not complete yet (its other query block comes with the next tile), block J - 1
