@@ -146,23 +146,28 @@ class TokenLogProbs(NamedTuple):
 MAX_TOP = 32
 
 
+def _token_logp(logits, tokens, top, keep):
+    """(logits and tokens as the kernel reads them, statistics for the backward pass when ``keep``, the four results)."""
+    x = logits if _row_padded(logits) else logits.contiguous()
+    N, C = x.shape
+    y, dev = tokens.contiguous(), x.device
+    logp, entropy = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
+    stat = torch.empty(2, N, dtype=torch.float32, device=dev) if keep else None   # row maximum, log of the row's sum above it
+    top_logp = torch.empty(N, top, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(N, top, dtype=torch.int64, device=dev)
+    with _lib.on_device(x):
+        rc = _lib.kernels().dtf_token_logp_fwd(_lib.ptr(x), _lib.ptr(y), _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp),
+                                               _lib.ptr(top_ids), _lib.ptr(stat), N, C,
+                                               ctypes.c_longlong(x.stride(0) if N > 1 else C), top, _lib.dtype_code(x.dtype),
+                                               _label_code(y), _lib.stream_ptr(dev))
+    _lib.check(rc, "token_logp_fwd")
+    return x, y, stat, logp, entropy, top_logp, top_ids
+
+
 class _TokenLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        x = logits if _row_padded(logits) else logits.contiguous()
-        N, C = x.shape
-        ld = x.stride(0) if N > 1 else C
-        y, dev = tokens.contiguous(), x.device
-        logp, entropy = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
-        stat = torch.empty(2, N, dtype=torch.float32, device=dev)        # row maximum, log of the row's sum above it
-        top_logp = torch.empty(N, top, dtype=torch.float32, device=dev)
-        top_ids = torch.empty(N, top, dtype=torch.int64, device=dev)
-        with _lib.on_device(x):
-            rc = _lib.kernels().dtf_token_logp_fwd(_lib.ptr(x), _lib.ptr(y), _lib.ptr(logp), _lib.ptr(entropy),
-                                                   _lib.ptr(top_logp), _lib.ptr(top_ids), _lib.ptr(stat), N, C,
-                                                   ctypes.c_longlong(ld), top, _lib.dtype_code(x.dtype), _label_code(y),
-                                                   _lib.stream_ptr(dev))
-        _lib.check(rc, "token_logp_fwd")
+        x, y, stat, logp, entropy, top_logp, top_ids = _token_logp(logits, tokens, top, True)
         ctx.save_for_backward(x, y, stat, entropy, top_ids)
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
@@ -225,7 +230,14 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) ->
         raise ValueError(f"top {top}: need 0 to {MAX_TOP}, and no more than the {V} logits of a row")
     if V < 1 or V > 1 << 30 or tokens.numel() >= 1 << 22:
         raise ValueError(f"{tokens.numel()} rows of {V} logits: need at least 1 logit a row and fewer than {1 << 22} rows")
-    x, y = logits.reshape(-1, V), tokens.reshape(-1)
-    run = _TokenLogp.apply if x.is_cuda and y.numel() else _token_logp_composed
-    r = run(x, y, int(top))
+    flat = tokens.dim() == 1
+    x, y = (logits, tokens) if flat else (logits.reshape(-1, V), tokens.reshape(-1))
+    if not (x.is_cuda and y.numel()):
+        r = _token_logp_composed(x, y, int(top))
+    elif x.requires_grad and torch.is_grad_enabled():
+        r = _TokenLogp.apply(x, y, int(top))
+    else:
+        r = _token_logp(x, y, int(top), False)[3:]
+    if flat:
+        return TokenLogProbs(*r)
     return TokenLogProbs(r[0].view(shape), r[1].view(shape), r[2].view(*shape, top), r[3].view(*shape, top))
