@@ -1592,7 +1592,7 @@ inline int dkdv_splits(int B, int Sk, int nh, int nkv) {
 
 // Workgroups of eight waves instead of four, whose two halves walk every other tile: for grids that leave the CUs with too
 // few waves to hide a tile's chain of products and exponentials. Otherwise the smaller ones fill the CUs better. Kernel
-// times in us, one / two halves, forward, dQ, dK / dV, heads of 64 if not said:
+// times in us in bf16, one / two halves, forward, dQ, dK / dV, heads of 64 if not said:
 //   at most a workgroup a CU: 4 x 512 x 12 heads 13.6 / 13.1, 15.7 / 15.4, 17.4 / 14.4; 2048 x 16 of 128 52 / 44, 67 / 56,
 //     111 / 100; more of them: 10 x 512 x 12 18 / 19, 21 / 28, 25 / 27, 16 x 512 x 12 26 / 28, 31 / 43, 35 / 44, 8 x 1000 keys
 //     x 10 of 80 (640 workgroups) dK / dV 39 / 47, 4 x 2048 causal x 16 of 128 94 / 103, 126 / 144, 184 / 248

@@ -67,9 +67,10 @@ def relative_bucket(distance: torch.Tensor, buckets: int, max_distance: int = 12
     return b + half * (d > 0) if bidirectional else b
 
 
+@lru_cache(maxsize=256)
 def _words(q_len: int, k_len: int, heads: int, q_start: int, buckets: int, max_distance: int, bidirectional: bool):
     w = (q_len, k_len, heads, q_start, buckets, max_distance, int(bidirectional),
-         *bucket_borders(buckets, max_distance, bidirectional))
+         *bucket_borders(buckets, max_distance, bidirectional))          # (the sizes of a call as its C entry reads them)
     return struct.pack(f"{len(w)}q", *w), len(w)
 
 

@@ -265,6 +265,23 @@ def test_table_gradient_of_bf16_attention_is_finer_than_bf16(Sq, masked):
     O.check("dtable", got, want, tol)
 
 
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("hd", [24, 64, 88, 128])
+@pytest.mark.parametrize("mode", ["plain", "causal_table", "key_bias"])
+def test_attention_of_more_workgroups_than_cus(dt, hd, mode):
+    """Grids beyond which a workgroup's waves walk the tiles together, over more than four tiles."""
+    B, Sq, Sk, nh, nkv = 8, 270, 390, 12, 12
+    q, k, v, do, table = _inputs(B, Sq, Sk, nh, nkv, hd, dt, 16)
+    if mode == "plain":
+        _compare(q, k, v, do, key_lengths=torch.tensor([390, 0, 389, 257, 64, 1, 300, 128]))
+    elif mode == "causal_table":
+        _compare(q, k, v, do, table, causal=True, rel_max_distance=40)
+    else:
+        bias = torch.randn(B, Sk, generator=torch.Generator().manual_seed(1))
+        bias[1], bias[2, 200:], bias[3, ::3] = -math.inf, -math.inf, -math.inf
+        _compare(q, k, v, do, table, key_bias=bias, rel_max_distance=300)
+
+
 def test_attention_over_a_cache_that_passes_32_bits():
     """Rows 2^22 elements apart (the widest that are read in place): the last ones lie 5 GB behind the first."""
     from distributed_tensorflow_amd.ops.attention import attention
