@@ -297,6 +297,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, un
   const unsigned bytes = left ? (unsigned)(left - 1) * row_bytes + bytes_per_row_used : 0u;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
 }
+// 8 consecutive elements of row r of a block of rows; zero outside the block, beyond the head size and where not `ok`: no
+// branch and no 64-bit address a row.
+__device__ __forceinline__ void block_row(Frag<unsigned short>& f, __amdgpu_buffer_rsrc_t rs, unsigned ld, int r, int e, bool ok) {
+  f.v = __builtin_bit_cast(bf16x8_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(ok ? (unsigned)r * ld + (unsigned)e * 2u : 0xffffffffu), 0, 0));
+}
+__device__ __forceinline__ void block_row(Frag<float>& f, __amdgpu_buffer_rsrc_t rs, unsigned ld, int r, int e, bool ok) {
+  const unsigned off = (unsigned)r * ld + (unsigned)e * 4u;
+  f.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(ok ? off : 0xffffffffu), 0, 0));
+  f.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(ok ? off + 16u : 0xffffffffu), 0, 0));
+}
 template <typename T, int D, int ROWS> struct Tile;
 template <int D, int ROWS>
 struct Tile<unsigned short, D, ROWS> {
@@ -1338,6 +1348,9 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
 
   Frag<T> kf[2][DS], vf[2][DS];
   float kbias[2];
+  const unsigned kld = (unsigned)a.k.ss * (unsigned)sizeof(T), vld = (unsigned)a.v.ss * (unsigned)sizeof(T), used = (unsigned)a.hd * (unsigned)sizeof(T);
+  const __amdgpu_buffer_rsrc_t krs = tile_rsrc(kp + (long long)k0 * a.k.ss, kld, used, klen - k0, 32);
+  const __amdgpu_buffer_rsrc_t vrs = tile_rsrc(vp + (long long)k0 * a.v.ss, vld, used, klen - k0, 32);
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
     const int k = k0 + kb * 16 + fr, kc = min(k, a.Sk - 1);
@@ -1347,8 +1360,16 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
 #pragma unroll
     for (int ks = 0; ks < DS; ++ks) {
       const int e = ks * 32 + g * 8;
-      frag_global(kf[kb][ks], kp + (long long)kc * a.k.ss, e, in && e < a.hd);
-      frag_global(vf[kb][ks], vp + (long long)kc * a.v.ss, e, in && e < a.hd);
+      if (D <= 64) {
+        // (with a load under a condition each, the row addresses do not fit the registers next to the fragments, and every
+        // load waits for the one before, the scratch memory being in between: 96 x 197 x 12 of 64 57 us, like this 48. The
+        // instances for 128 come out with slower loops like this: 4 x 2048 causal 182 and 210)
+        block_row(kf[kb][ks], krs, kld, kb * 16 + fr, e, in && e < a.hd);
+        block_row(vf[kb][ks], vrs, vld, kb * 16 + fr, e, in && e < a.hd);
+      } else {
+        frag_global(kf[kb][ks], kp + (long long)kc * a.k.ss, e, in && e < a.hd);
+        frag_global(vf[kb][ks], vp + (long long)kc * a.v.ss, e, in && e < a.hd);
+      }
     }
   }
   f32x4 dk[DB][2], dv[DB][2];
