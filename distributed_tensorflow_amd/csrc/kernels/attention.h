@@ -17,8 +17,8 @@
 // as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score.
 //
 // Measured (bf16, us and the rate of the products): 64 x 512 tokens x 12 heads of 64, with a table: forward 111 (P in two
-// parts, see PARTS), dQ and dTable 174, dK / dV 157; without one 85, 111, 133 (610, 695, 775 TFLOP/s of what each has to do);
-// 4 x 8192 x 12 of 64, not causal: 955, 1243, 1265 TFLOP/s; 4 x 2048 causal, 16 heads on 4 of 128: 94, 125, 183 and 24 for
+// parts, see PARTS), dQ and dTable 174, dK / dV 157; without one 85, 111, 120 (605, 697, 862 TFLOP/s of what each has to do);
+// 4 x 8192 x 12 of 64, not causal: 893, 1206, 1237 TFLOP/s; 4 x 2048 causal, 16 heads on 4 of 128: 94, 125, 183 and 24 for
 // the join. Long rows are bound by the vector instructions beside the products (the forward pass keeps them 70 % busy:
 // maximum, exponential, sum, conversion of every score); at 512 tokens and less by a workgroup's beginning and end, where
 // it waits for memory.
