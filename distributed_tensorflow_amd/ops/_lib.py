@@ -16,6 +16,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_DIR = Path(__file__).resolve().parent.parent / "lib"
 _kernels = None
@@ -115,6 +116,25 @@ _here = contextlib.nullcontext()
 def on_device(t: torch.Tensor):
     """Makes ``t``'s GPU the current one for a launch on it (the kernels use the current device's context)."""
     return _here if t.device.index == torch.cuda.current_device() else _device(t)
+
+
+_tracing, _mode, _proxies = torch._C._get_tracing_state, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+
+
+def differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these has to go through its autograd function rather than straight to the kernels: a gradient is
+    asked for, or a level of forward-mode derivatives is open. The functions have no forward derivative, so one that is given
+    a tangent raises; the kernels alone would drop it. A call in a trace is refused: what they write is no operation that a
+    trace holds, and it would return memory that nothing wrote."""
+    if _tracing() is not None or _mode(_proxies) is not None:
+        raise RuntimeError("the kernels cannot be part of a trace: torch.jit.trace and make_fx would record none of their work")
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

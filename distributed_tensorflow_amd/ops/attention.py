@@ -379,8 +379,7 @@ def _general(q, k, v, nkv, key_bias, causal, scale, key_lengths, q_start, rel_ta
     opts = (bool(causal), scale, start0, int(rel_max_distance), bidirectional)
     if not q.is_cuda:
         return _composed(q, k, v, rel_table, key_bias, lens, starts, nkv, opts)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and (k.requires_grad or v.requires_grad))
-                                    or (rel_table is not None and rel_table.requires_grad)):
+    if _lib.differentiated(q, k, v, rel_table):
         return _GeneralFn.apply(q, k, v, rel_table, key_bias, lens, starts, nkv, opts)
     return _forward(q, k, v, rel_table, key_bias, lens, starts, nkv, opts, None, None)[0]
 
@@ -403,7 +402,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_bias: torch
     ``rel_table[buckets, nh]`` adds the learned bias of ``ops/relative_bias.py`` for the distance to that position
     (``rel_bidirectional`` defaults to ``not causal``). A query that no key is left for gets zeros, and zero gradients.
 
-    K and V of keys that only ``causal`` hides have to be finite."""
+    K and V of keys that only ``causal`` hides have to be finite. On a GPU forward-mode derivatives and traces are refused."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError(f"q[B, Sq, nh, hd] and k, v[B, Sk, nkv, hd] do not fit: {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")

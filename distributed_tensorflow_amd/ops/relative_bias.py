@@ -116,13 +116,13 @@ def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: 
     """``[heads, q_len, k_len]`` bias, in the type of ``table`` (``[buckets, heads]``, float32 or bfloat16).
 
     ``q_start`` is the position of the first query counted from the first key; by default the queries are the last
-    ``q_len`` of the ``k_len`` positions (0 for self-attention)."""
+    ``q_len`` of the ``k_len`` positions (0 for self-attention). On a GPU forward-mode derivatives and traces are refused."""
     check_buckets(table, None, max_distance, bidirectional)
     q_start = k_len - q_len if q_start is None else int(q_start)
     if q_len < 0 or k_len < 0 or max(q_len, k_len) > 1 << 28 or abs(q_start) > 1 << 29:
         raise ValueError(f"lengths {q_len} and {k_len} with the first query at {q_start} are out of range")
     if table.is_cuda:
-        run = _BiasFn.apply if table.requires_grad and torch.is_grad_enabled() else _forward
+        run = _BiasFn.apply if _lib.differentiated(table) else _forward
         return run(table, q_len, k_len, q_start, max_distance, bool(bidirectional))
     d = torch.arange(k_len)[None, :] - (torch.arange(q_len)[:, None] + q_start)
     return table.t()[:, relative_bucket(d, table.shape[0], max_distance, bidirectional)]

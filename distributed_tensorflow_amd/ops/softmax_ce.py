@@ -218,7 +218,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) ->
 
     A token outside ``[0, V)`` (an ignored position) has ``logp`` 0 and no gradient through it. Alternatives of equal
     logits come lowest index first. Logits of -inf are words that cannot be; in a row of nothing else the log
-    probabilities are -inf, the entropy 0 and the gradients 0. The three floating results have gradients."""
+    probabilities are -inf, the entropy 0 and the gradients 0. The three floating results have gradients; on a GPU
+    forward-mode derivatives and traces are refused."""
     if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
         raise ValueError(f"logits [..., V] and tokens [...] do not fit: {tuple(logits.shape)}, {tuple(tokens.shape)}")
     if logits.device != tokens.device:
@@ -234,7 +235,7 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) ->
     x, y = (logits, tokens) if flat else (logits.reshape(-1, V), tokens.reshape(-1))
     if not (x.is_cuda and y.numel()):
         r = _token_logp_composed(x, y, int(top))
-    elif x.requires_grad and torch.is_grad_enabled():
+    elif _lib.differentiated(x):
         r = _TokenLogp.apply(x, y, int(top))
     else:
         r = _token_logp(x, y, int(top), False)[3:]

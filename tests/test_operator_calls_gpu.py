@@ -1,0 +1,53 @@
+"""Calls of general attention, relative position bias and token log probabilities that their documentation allows beyond the
+ordinary ones, on the GPU against the 64-bit oracles (bounds: operator_oracles.py)."""
+import os
+import sys
+
+import pytest
+import torch
+from torch.autograd import forward_ad as fwAD
+
+sys.path.insert(0, os.path.dirname(__file__))
+from test_operators_gpu import DEV, FP32, _inputs  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------ tangents and traces
+def _one_call_each():
+    """(name, its differentiable inputs, call)"""
+    from distributed_tensorflow_amd.ops.attention import attention, self_attention
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    from distributed_tensorflow_amd.ops.softmax_ce import token_log_probs
+    q, k, v, _, table = (t.to(DEV) for t in _inputs(2, 40, 50, 2, 1, 16, FP32, 8))
+    few = q[:, :1].contiguous()
+    bias = torch.zeros(2, 50, device=DEV)
+    x, tok = torch.randn(6, 40, device=DEV), torch.arange(6, device=DEV)
+    return [("attention", (q, k, v, bias, table), lambda q, k, v, b, t: attention(q, k, v, b, rel_table=t)),
+            ("attention, few queries", (few, k, v, bias, table), lambda q, k, v, b, t: attention(q, k, v, b, rel_table=t)),
+            ("self_attention", (k.repeat(1, 1, 4, 1), table), lambda x, t: self_attention(x, kv_heads=1, rel_table=t)),
+            ("relative_bias", (table,), lambda t: relative_bias(t, 9, 12)),
+            ("token_log_probs", (x,), lambda x: token_log_probs(x, tok, 3).logp)]
+
+
+def test_a_tangent_is_refused_and_not_dropped():
+    for name, ins, call in _one_call_each():
+        want = call(*ins)
+        for i in range(len(ins)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), fwAD.dual_level():
+                    with pytest.raises(NotImplementedError):
+                        call(*ins[:i], fwAD.make_dual(ins[i], torch.ones_like(ins[i])), *ins[i + 1:])
+                    assert torch.equal(call(*ins), want), name             # (a level without a tangent changes nothing)
+        assert torch.equal(call(*ins), want), name
+
+
+def test_a_trace_is_refused_and_not_left_without_the_kernels():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for name, ins, call in _one_call_each():
+        for trace in (lambda: torch.jit.trace(call, ins), lambda: make_fx(call)(*ins)):
+            with pytest.raises(RuntimeError, match="trace"):
+                trace()
+        call(*ins)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (ins[0].detach().clone().requires_grad_(), *ins[1:]))
