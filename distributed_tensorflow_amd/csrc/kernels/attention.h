@@ -13,8 +13,11 @@
 // v_mfma_f32_16x16x4_f32, eight of which cover the same 32 contraction elements (Frag below holds 8 elements of a lane
 // for either type; the order of the 32 elements is free as long as both operands agree on it).
 //
-// Scores are kept in units of 1 / (scale log2 e): the biases are divided by that factor where they are staged and enter
-// as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score.
+// Scores are kept as step t for a factor step = unit / scale (unit 1: q . k as it is): the biases are multiplied by it where
+// they are staged and enter as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score.
+// Beside a key bias unit is the power of two below a scale under 1, and the operand that stays in registers carries it: step
+// is then at most 1, so any finite bias stays finite, and equal ones equal (1 / scale itself would carry a bias beyond 4.3e37
+// past the type's range at heads of 64). A power of two rounds nothing.
 //
 // Measured (bf16, us and the rate of the products): 64 x 512 tokens x 12 heads of 64, with a table: forward 111 (P in two
 // parts, see PARTS), dQ and dTable 174, dK / dV 157; without one 85, 111, 120 (605, 697, 862 TFLOP/s of what each has to do);
@@ -58,7 +61,8 @@ struct Args {
   unsigned char* fine;               // bf16: [B, Sq, nh, hd] the next 8 bits of O, for D (see finer); or null
   float* part;                       // partial results of the key splits (few queries), of the head splits (dK / dV)
   int B, Sq, Sk, nh, nkv, hd, causal, splits, ksplits;
-  float scale, inv_scale;
+  float scale;                       // of the formula: dQ and dK are multiplied by it
+  float unit, score_scale, step;     // t = score_scale * score, score = unit q . k + step * biases; step = 1 / score_scale
 };
 
 // What the dK / dV kernel wants of each query, in tiles of 64 that one direct load of 1 KiB brings to the LDS: the row
@@ -112,6 +116,17 @@ __device__ __forceinline__ void pack(Frag<unsigned short>& f, const f32x4& a, co
   f.v = __builtin_bit_cast(bf16x8_t, r);
 }
 __device__ __forceinline__ void pack(Frag<float>& f, const f32x4& a, const f32x4& b) { f.lo = a; f.hi = b; }
+// times a power of two
+__device__ __forceinline__ void times(Frag<unsigned short>& f, float by) {
+  u32x4_t r = __builtin_bit_cast(u32x4_t, f.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = pack_bf16x2(__uint_as_float(r[i] << 16) * by, __uint_as_float(r[i] & 0xffff0000u) * by);
+  f.v = __builtin_bit_cast(bf16x8_t, r);
+}
+__device__ __forceinline__ void times(Frag<float>& f, float by) {
+  f.lo *= by;
+  f.hi *= by;
+}
 // what pack() rounded off
 __device__ __forceinline__ void pack_rest(Frag<unsigned short>& f, f32x4 a, f32x4 b, const Frag<unsigned short>& packed) {
   const u32x4_t r = __builtin_bit_cast(u32x4_t, packed.v);
@@ -403,19 +418,14 @@ __device__ __forceinline__ float table_at(const Args& a, int bucket, int h) {
   const long long i = (long long)bucket * a.nh + h;
   return a.table_bf16 ? bf16_to_f32(((const unsigned short*)a.table)[i]) : ((const float*)a.table)[i];
 }
-// Biases in score units. A key bias is a mask as well: a finite one stays finite, and so does its product with
-// scale log2 e, so it is never taken for -inf. A learned value is held to +-2^24 powers of two (beyond that the scores
-// next to it would be lost in fp32 anyway), so that the kernels without key bias may take the maximum off by one fma.
-__device__ __forceinline__ float to_score_units(const Args& a, float bias) {
-  const float lim = 3.0e38f / fmaxf(1.f, a.scale * kLog2e);
-  const float v = bias * a.inv_scale;
-  if (bias == -INFINITY) return bias;
-  return v < -lim ? -lim : v;        // NaN and +inf pass
-}
+// Biases in score units. A key bias is a mask as well: only -inf is one, and a finite one stays finite, as step <= 1 beside
+// key biases. A learned value is held to +-2^24 powers of two (beyond that the scores next to it would be lost in fp32
+// anyway), so that the kernels without key bias may take the maximum off by one fma.
+__device__ __forceinline__ float to_score_units(const Args& a, float bias) { return bias * a.step; }
 __device__ __forceinline__ float learned_bias(const Args& a, float bias) {
   if (bias == -INFINITY || bias == INFINITY) return bias;
   const float lim = 16777216.f / kLog2e, v = bias > lim ? lim : bias < -lim ? -lim : bias;
-  return v * a.inv_scale;
+  return v * a.step;
 }
 __device__ __forceinline__ void fill_band(const Args& a, int h, float* band, int tid) {
   const int n = band_size(a);
@@ -498,7 +508,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
   const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
   const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
   const int pos0 = start + q0;
-  const float c = a.scale * kLog2e;
+  const float c = a.score_scale * kLog2e;
   const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
   const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
   const bool rel = MODE == kRel || (MODE == kKeys && a.table);
@@ -508,7 +518,10 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
   for (int qb = 0; qb < 2; ++qb) {
     const T* row = qp + (long long)min(q0 + qb * 16 + fr, a.Sq - 1) * a.q.ss;
 #pragma unroll
-    for (int ks = 0; ks < DS; ++ks) frag_global(qf[qb][ks], row, ks * 32 + g * 8, ks * 32 + g * 8 < a.hd);
+    for (int ks = 0; ks < DS; ++ks) {
+      frag_global(qf[qb][ks], row, ks * 32 + g * 8, ks * 32 + g * 8 < a.hd);
+      if (MODE == kKeys) times(qf[qb][ks], a.unit);
+    }
   }
   f32x4 o[DB][2];
 #pragma unroll
@@ -761,7 +774,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
   const int bk = uni(blockIdx.x / a.splits), split = blockIdx.x - bk * a.splits, b = uni(bk / a.nkv), kvh = bk - b * a.nkv;
   const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
   const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
-  const float c = a.scale * kLog2e;
+  const float c = a.score_scale * kLog2e;
   const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
   const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
@@ -785,7 +798,10 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
     pos[qb] = start + i;
     tb[qb] = tab + hg * a.buckets;
 #pragma unroll
-    for (int ks = 0; ks < DS; ++ks) frag_global(qf[qb][ks], row, ks * 32 + g * 8, ks * 32 + g * 8 < a.hd);
+    for (int ks = 0; ks < DS; ++ks) {
+      frag_global(qf[qb][ks], row, ks * 32 + g * 8, ks * 32 + g * 8 < a.hd);
+      if (MODE == kKeys) times(qf[qb][ks], a.unit);
+    }
   }
   f32x4 o[DB][QB];
 #pragma unroll
@@ -960,7 +976,7 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a) {
   __shared__ float fac[64], stats[2];
   const int group = a.nh / a.nkv, rows = a.Sq * group, tid = threadIdx.x;
   const long long row = blockIdx.x, n_rows = gridDim.x;
-  const float c = a.scale * kLog2e;
+  const float c = a.score_scale * kLog2e;
   const float* st = a.part + (long long)a.splits * n_rows * D;
   const int sub = tid / L, d = (tid - sub * L) * 4;
   if (tid < 64) {                                        // (at most 64 splits)
@@ -1068,7 +1084,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
   const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
   const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
   const int pos0 = start + q0;
-  const float c = a.scale * kLog2e;
+  const float c = a.score_scale * kLog2e;
   const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
   const T* op = (const T*)a.out.p + b * a.out.sb + h * a.out.sh;
   const T* dop = (const T*)a.dout.p + b * a.dout.sb + h * a.dout.sh;
@@ -1095,6 +1111,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
       } else {
         part = dot(of, dof[qb][ks], part);
       }
+      if (MODE == kKeys) times(qf[qb][ks], a.unit);
     }
     const long long i = ((long long)b * a.nh + h) * a.Sq + qc, n = (long long)a.B * a.nh * a.Sq;
     dl[qb] = group_sum(part);
@@ -1339,7 +1356,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
   const int heads = uni(group / a.ksplits), kb0 = rank * kRows, k0 = kb0 + wid * 32;
   const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
   const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
-  const float c = a.scale * kLog2e;
+  const float c = a.score_scale * kLog2e;
   const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
   const float* kbp = MODE == kKeys ? a.key_bias + (long long)b * a.Sk : nullptr;
@@ -1370,6 +1387,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
         frag_global(kf[kb][ks], kp + (long long)kc * a.k.ss, e, in && e < a.hd);
         frag_global(vf[kb][ks], vp + (long long)kc * a.v.ss, e, in && e < a.hd);
       }
+      if (MODE == kKeys) times(kf[kb][ks], a.unit);
     }
   }
   f32x4 dk[DB][2], dv[DB][2];

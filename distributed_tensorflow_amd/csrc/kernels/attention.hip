@@ -4,6 +4,8 @@
 // what the kernels assume and returns a negative code without launching anything when it does not hold.
 #include "attention.h"
 
+#include <cmath>
+
 using namespace dtf;
 
 namespace {
@@ -45,8 +47,14 @@ bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   a.causal = (int)w[kCausal];
   a.part = (float*)w[kPart];
   a.fine = (unsigned char*)w[kFine];
-  a.scale = scale;
-  a.inv_scale = 1.f / scale;
+  a.scale = a.score_scale = scale;
+  a.unit = 1.f;
+  if (a.key_bias && scale < 1.f) {                       // score_scale in [1, 2)
+    int e = 0;
+    a.score_scale = 2.f * std::frexp(scale, &e);
+    a.unit = std::ldexp(1.f, e - 1);
+  }
+  a.step = 1.f / a.score_scale;
   if (!(scale > 0.f) || scale > 1e30f || a.hd % 8 || a.hd > 128 || a.nh % a.nkv) return false;
   if (a.table) {
     a.n_thr = a.half - a.exact - 1;

@@ -1,5 +1,6 @@
 """Calls of general attention, relative position bias and token log probabilities that their documentation allows beyond the
 ordinary ones, on the GPU against the 64-bit oracles (bounds: operator_oracles.py)."""
+import math
 import os
 import sys
 
@@ -8,7 +9,7 @@ import torch
 from torch.autograd import forward_ad as fwAD
 
 sys.path.insert(0, os.path.dirname(__file__))
-from test_operators_gpu import DEV, FP32, _inputs  # noqa: E402
+from test_operators_gpu import BF16, DEV, FP32, _compare, _inputs  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +52,34 @@ def test_a_trace_is_refused_and_not_left_without_the_kernels():
         call(*ins)
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(call, (ins[0].detach().clone().requires_grad_(), *ins[1:]))
+
+
+# ------------------------------------------------------------------------------------------ key biases at the ends of their type
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Sq,Sk", [(70, 90), (3, 700)], ids=["rows", "few"])
+@pytest.mark.parametrize("scale", [None, 0.3, 3.0, 1e-3])
+@pytest.mark.parametrize("rel", [0, 8])
+def test_attention_key_biases_of_any_finite_value(dt, Sq, Sk, scale, rel):
+    """The largest value on one key and on several, large ones of both signs, and rows of lowest values of two types."""
+    q, k, v, do, table = _inputs(5, Sq, Sk, 4, 2, 40, dt, rel, seed=2)
+    kb = torch.zeros(5, Sk)
+    kb[0, 17] = torch.finfo(FP32).max
+    kb[1, 3:60:7] = torch.finfo(FP32).max
+    kb[1, 5], kb[1, 9] = -math.inf, torch.finfo(FP32).min
+    kb[2, ::2], kb[2, 1::2] = 1e37, 2e38
+    kb[3], kb[3, 11:40:3] = torch.finfo(FP32).min, torch.finfo(BF16).min
+    kb[4, :] = -1e38
+    kb[4, Sk // 2:] = -3e38
+    _compare(q, k, v, do, table, key_bias=kb, scale=scale, rel_max_distance=20)
+
+
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Sq", [70, 3], ids=["rows", "few"])
+def test_attention_key_biases_beside_the_smallest_scale(dt, Sq):
+    """scale 2e-30: the biases alone decide, ordinary ones and those that 1 / scale would carry past the type."""
+    q, k, v, do, _ = _inputs(3, Sq, 300, 2, 2, 16, dt, seed=6)
+    kb = torch.randn(3, 300, generator=torch.Generator().manual_seed(1))
+    kb[1, 40:50] = torch.arange(10.0) * 1e31
+    kb[2] = -1e31
+    kb[2, 7::2] = -2e31
+    _compare(q, k, v, do, key_bias=kb, scale=2e-30)
