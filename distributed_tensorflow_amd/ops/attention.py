@@ -362,6 +362,9 @@ def _general(q, k, v, nkv, key_bias, causal, scale, key_lengths, q_start, rel_ta
             raise ValueError(f"key_bias is a floating tensor [{B}, {Sk}] on {q.device}, got {tuple(key_bias.shape)}")
         if key_bias.requires_grad:
             raise ValueError("key_bias has no gradient: pass it detached")
+        if key_bias.dtype == torch.float64:        # (a finite bias that 32 bits do not hold is none of their infinities)
+            top = torch.finfo(torch.float32).max
+            key_bias = torch.where(key_bias.isinf(), key_bias, key_bias.clamp(-top, top))
         key_bias = key_bias.float().contiguous()
     lens = None if key_lengths is None else _int_vector(key_lengths, "key_lengths", B, q.device)
     starts, start0 = None, Sk - Sq

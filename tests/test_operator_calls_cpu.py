@@ -29,3 +29,17 @@ def test_traces_are_refused():
         with pytest.raises(RuntimeError, match="trace"):
             trace()
     call(x)
+
+
+def test_attention_key_bias_in_64_bits():
+    """A finite bias that 32 bits do not hold masks nothing: its keys share the row where no other is left."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    q, k, v = (torch.randn(2, n, 2, 16, generator=torch.Generator().manual_seed(n)) for n in (3, 9, 9))
+    bias = torch.zeros(2, 9, dtype=torch.float64)
+    bias[0] = torch.finfo(torch.float64).min
+    bias[0, 4], bias[1, 2] = -torch.inf, torch.finfo(torch.float64).max
+    out = attention(q, k, v, bias)
+    alone = bias[0] != -torch.inf
+    # a mean of 8 numbers: 8 roundings of 2^-24 of their magnitudes, and the softmax's few
+    assert float((out[0] - v[0, alone].mean(0)).abs().max()) <= 32 * 2.0 ** -24 * float(v.abs().max())
+    assert torch.equal(out[1], v[1, 2].expand(3, 2, 16))

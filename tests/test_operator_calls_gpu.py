@@ -83,3 +83,16 @@ def test_attention_key_biases_beside_the_smallest_scale(dt, Sq):
     kb[2] = -1e31
     kb[2, 7::2] = -2e31
     _compare(q, k, v, do, key_bias=kb, scale=2e-30)
+
+
+# ------------------------------------------------------------------------------------------ key biases in 64 bits
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Sq", [70, 3], ids=["rows", "few"])
+def test_attention_key_bias_in_64_bits(dt, Sq):
+    """float64's lowest value is finite: no mask, whatever 32 bits make of it."""
+    q, k, v, do, _ = _inputs(2, Sq, 300, 2, 2, 16, dt, seed=7)
+    kb = torch.zeros(2, 300, dtype=torch.float64)
+    kb[0] = torch.finfo(torch.float64).min
+    kb[1, 40:50] = torch.finfo(torch.float64).max
+    kb[1, 60] = -math.inf
+    _compare(q, k, v, do, key_bias=kb)
