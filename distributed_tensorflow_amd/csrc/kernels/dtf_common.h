@@ -70,6 +70,12 @@ __device__ __forceinline__ void store16_through(void* p, u32x4_t v) {
   asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1" ::"v"(p), "v"(v) : "memory");
 }
 __device__ __forceinline__ void drain_stores() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// What the lanes of a wave wrote before is what they read after, in the LDS. The hardware serves a wave's LDS instructions in
+// order anyway; this keeps the compiler, which sees one lane at a time, from reordering them. No instruction comes of it.
+__device__ __forceinline__ void wave_ordered() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

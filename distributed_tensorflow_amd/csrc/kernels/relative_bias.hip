@@ -101,7 +101,9 @@ __device__ __forceinline__ void load8(const float* row, int j, int n, float (&o)
 // A wave takes tiles of 8 rows x 512 columns, a lane 8 x 8 of them: 64 elements on 15 diagonals, which it adds up in
 // registers. Where the 15 distances are all on one far side (most of a long row) they go into one register; on the band
 // they go to the wave's own LDS sums, 15 additions with the lanes 8 distances apart (the sums are stored by distance
-// modulo 8 first, so that they fall on neighbouring banks). No sum depends on another wave: the order is fixed.
+// modulo 8 first, so that they fall on neighbouring banks). No sum depends on another wave: the order is fixed. Additions 0
+// to 7 of a tile meet no word twice, nor do 8 to 14, but a lane's second eight are its neighbour's first: between the two, and
+// between tiles, wave_ordered() keeps the compiler from moving one lane's read before another's write.
 template <typename T>
 __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, const T* __restrict__ g, float* __restrict__ parts,
                                                        int tiles_per_wave, int col_tiles, long long n_tiles) {
@@ -110,6 +112,7 @@ __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, const T* __re
   const int n = a.max_dist + a.right + 1, eighth = (n + 14) / 8 + 1, size = eighth * 8;   // distances -max_dist - 7 ..
   float* sums = reinterpret_cast<float*>(smem) + wid * size;
   for (int i = lane; i < size; i += 64) sums[i] = 0.f;
+  wave_ordered();
   float far_l = 0.f, far_r = 0.f;
   const long long first = ((long long)blockIdx.x * 4 + wid) * tiles_per_wave;
   for (long long t = first; t < first + tiles_per_wave && t < n_tiles; ++t) {
@@ -142,8 +145,10 @@ __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, const T* __re
         if (low + d <= -a.max_dist) far_l += acc[d];
         else if (low + d >= a.right) far_r += acc[d];
         else sums[(i & 7) * eighth + (i >> 3)] += acc[d];
+        if (d == 7) wave_ordered();
       }
     }
+    wave_ordered();
   }
   __shared__ float scratch[16];
   far_l = block_sum(far_l, scratch);

@@ -9,6 +9,7 @@ import torch
 from torch.autograd import forward_ad as fwAD
 
 sys.path.insert(0, os.path.dirname(__file__))
+import operator_oracles as O  # noqa: E402
 from test_operators_gpu import BF16, DEV, FP32, _compare, _inputs  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,54 @@ def test_attention_key_bias_in_64_bits(dt, Sq):
     kb[1, 40:50] = torch.finfo(torch.float64).max
     kb[1, 60] = -math.inf
     _compare(q, k, v, do, key_bias=kb)
+
+
+# ------------------------------------------------------------------------------------------ the written bias
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cfg", [(3001, 2999, 20, 32, 128, True, None), (4099, 1501, 24, 16, 50, False, -900),
+                                 (1203, 5003, 17, 128, 2048, True, 1700), (60007, 33, 3, 8, 8, True, -20000)], ids=str)
+def test_relative_bias_gradient_of_several_tiles_a_wave(dt, cfg):
+    """heads x tiles (8 rows x 512 columns) beyond twice 8192, so that a wave walks several of them, at odd lengths and with a
+    last wave whose share is short. The sums are made in 64 bits on the GPU, diagonal by diagonal; bound as the oracle's,
+    with the terms that a wave adds up in a row: a register takes 64 elements of each tile, an LDS sum 15."""
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    q_len, k_len, heads, buckets, far, bidir, start = cfg
+    tiles = -(-q_len // 8) * -(-k_len // 512)
+    per = tiles * heads // 8192
+    assert per >= 2 and tiles % per
+    g = torch.Generator(DEV).manual_seed(q_len)
+    table = torch.randn(buckets, heads, device=DEV, generator=g).to(dt).requires_grad_()
+    do = torch.randn(heads, q_len, k_len, device=DEV, generator=g).to(dt)
+    first = k_len - q_len if start is None else start
+    out = relative_bias(table, q_len, k_len, max_distance=far, bidirectional=bidir, q_start=start)
+    got, = torch.autograd.grad(out, table, do)
+    low = -(q_len - 1) - first
+    of = O.buckets_between(low, k_len - 1 - first, buckets, far, bidir).to(DEV)
+    assert torch.equal(out[0], table[:, 0][of].unfold(0, k_len, 1).flip(0))
+    where = (torch.arange(k_len, device=DEV)[None] - torch.arange(q_len, device=DEV)[:, None] + (q_len - 1)).flatten()
+    want, mag = (torch.zeros(buckets, heads, dtype=torch.float64, device=DEV) for _ in range(2))
+    for h in range(heads):
+        x = do[h].flatten().double()
+        for w, y in ((want, x), (mag, x.abs())):
+            diag = torch.zeros(q_len + k_len - 1, dtype=torch.float64, device=DEV).index_add_(0, where, y)
+            w[:, h].index_add_(0, of, diag)
+    tol = (64 * per + 4096) * O.U32 * mag + O.half_step(dt) * want.abs()
+    O.check("dtable", got, want.cpu(), 1.01 * tol.cpu() + 1e-30)
+    again, = torch.autograd.grad(relative_bias(table, q_len, k_len, max_distance=far, bidirectional=bidir, q_start=start), table, do)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+def test_relative_bias_of_more_rows_than_a_grid(dt):
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    q_len, k_len, heads, buckets = 140001, 37, 2, 32
+    table = torch.randn(buckets, heads, generator=torch.Generator().manual_seed(1)).to(dt).to(DEV).requires_grad_()
+    out = relative_bias(table, q_len, k_len, q_start=-70000)
+    of = O.buckets_between(-(q_len - 1) + 70000, k_len - 1 + 70000, buckets, 128, True).to(DEV)
+    for h in range(heads):
+        assert torch.equal(out[h], table[:, h][of].unfold(0, k_len, 1).flip(0)), h
+    # (a gradient of ones counts a bucket's elements: whole numbers below 2^24, summed exactly, rounded once)
+    count = torch.bincount(of, torch.minimum(torch.minimum(torch.arange(1, q_len + k_len, device=DEV), torch.tensor(k_len, device=DEV)),
+                                             torch.arange(q_len + k_len - 1, 0, -1, device=DEV)).double(), minlength=buckets)
+    got, = torch.autograd.grad(out, table, torch.ones_like(out))
+    assert torch.equal(got, count[:, None].expand(-1, heads).to(dt))
