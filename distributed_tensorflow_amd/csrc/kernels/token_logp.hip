@@ -98,14 +98,16 @@ struct Shared {
   float red[3][16];
 };
 
-// The k best of cand[0 .. n) and best[0 .. nb), by counting the greater ones: one wave.
+// The k best of cand[0 .. n) and best[0 .. nb), by counting the greater ones: one wave. Its lanes read what others wrote.
 __device__ __forceinline__ void rank_candidates(Shared& sh, int n, int nb, int k, int lane) {
   const int total = n + nb;
   if (total <= 64) {                                     // almost always
     const u64 mine = lane < n ? sh.cand[lane] : (lane < total ? sh.best[lane - n] : 0ull);
     int rank = 0;
     for (int j = 0; j < total; ++j) rank += lane_u64(mine, j) > mine ? 1 : 0;
+    wave_ordered();
     if (lane < total && rank < k) sh.best[rank] = mine;
+    wave_ordered();
     return;
   }
   for (int c = 0; c < total; c += 64) {
@@ -115,7 +117,9 @@ __device__ __forceinline__ void rank_candidates(Shared& sh, int n, int nb, int k
     for (int j = 0; j < total; ++j) rank += (j < n ? sh.cand[j] : sh.best[j - n]) > mine ? 1 : 0;
     if (i < total && rank < k) sh.sorted[rank] = mine;
   }
+  wave_ordered();
   if (lane < (total < k ? total : k)) sh.best[lane] = sh.sorted[lane];
+  wave_ordered();
 }
 
 template <typename T, typename L, int NT, bool TOP>
@@ -270,8 +274,10 @@ __global__ __launch_bounds__(NT, 6) void token_logp_fwd_kernel(const T* __restri
       // Those held from earlier chunks stay, before the ones that come again
       if (wid == 0) {
         const u64 kept = lane < nb ? sh.best[lane] : 0ull;
+        wave_ordered();
         rank_candidates(sh, kCap, nb, k, lane);
         if (lane == 0) sh.threshold = sh.best[k - 1];
+        wave_ordered();
         if (lane < nb) sh.best[lane] = kept;
         if (lane == 0) sh.count = held;
       }

@@ -10,7 +10,7 @@ from torch.autograd import forward_ad as fwAD
 
 sys.path.insert(0, os.path.dirname(__file__))
 import operator_oracles as O  # noqa: E402
-from test_operators_gpu import BF16, DEV, FP32, _compare, _inputs  # noqa: E402
+from test_operators_gpu import BF16, DEV, FP32, _compare, _compare_logp, _inputs, _logits  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,17 @@ def test_relative_bias_of_more_rows_than_a_grid(dt):
                                              torch.arange(q_len + k_len - 1, 0, -1, device=DEV)).double(), minlength=buckets)
     got, = torch.autograd.grad(out, table, torch.ones_like(out))
     assert torch.equal(got, count[:, None].expand(-1, heads).to(dt))
+
+
+# ------------------------------------------------------------------------------------------ token log probabilities
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+def test_token_log_probs_of_subnormal_logits(dt):
+    """Logits below the smallest normal number, of both signs: their order is that of the values all the same."""
+    x, tok, g = _logits(6, 5003, dt)
+    tiny = torch.finfo(dt).tiny
+    x[0] = (torch.randn(5003, generator=g) * tiny / 8).to(dt)
+    x[1] = -(torch.rand(5003, generator=g) * tiny / 8).to(dt)
+    x[2, 100:] = -tiny / 4
+    x[2, :100] = -tiny / 2
+    gs = (torch.randn(6, generator=g), torch.randn(6, generator=g), torch.randn(6, 9, generator=g))
+    _compare_logp(x, tok, 9, gs)
