@@ -86,10 +86,13 @@ attn::Run instance(const attn::Args& a, bool bf16) {
   return bf16 ? attn::run_bf16_plain : attn::run_f32_plain;
 }
 
-bool grid_ok(const attn::Args& a) {
-  const long long q = (long long)a.B * a.nh * ((a.Sq + attn::kRows - 1) / attn::kRows);
-  const long long k = (long long)a.B * a.nh * ((a.Sk + attn::kRows - 1) / attn::kRows);
-  return q < (1LL << 31) / 256 && k < (1LL << 31) / 256;
+// Grids of the kernels that the call launches: fewer than 2^32 threads, at most 512 a workgroup. (Where keys or heads are
+// split, there are fewer than 768 workgroups without the splits: those grids and the joins' stay far below.)
+bool grid_ok(const attn::Args& a, bool backward) {
+  const long long most = 1LL << 23;
+  if (backward && (long long)a.B * a.nkv * ((a.Sk + attn::kRows - 1) / attn::kRows) >= most) return false;
+  if (!backward && attn::few_queries(a.Sq, a.nh, a.nkv)) return (long long)a.B * a.nkv < most;
+  return (long long)a.B * a.nh * ((a.Sq + attn::kRows - 1) / attn::kRows) < most;
 }
 
 // dtable[u, h] = sum over the parts, in a fixed order: one workgroup a head, its threads split the parts.
@@ -129,7 +132,7 @@ DTF_API int dtf_attention_fwd(const long long* words, int n_words, float scale, 
   if (!unpack(words, n_words, scale, a)) return -1;
   const bool bf16 = words[kBf16];
   if (!operands_ok(a, bf16 ? 2 : 4, false)) return -2;
-  if (!grid_ok(a)) return -3;
+  if (!grid_ok(a, false)) return -3;
   a.splits = dtf_attention_splits(a.B, a.Sq, a.Sk, a.nh, a.nkv);
   if (a.splits > 1 && !a.part) return -5;
   return instance(a, bf16)(a, false, stream);
@@ -141,7 +144,7 @@ DTF_API int dtf_attention_bwd(const long long* words, int n_words, float scale, 
   if (!unpack(words, n_words, scale, a)) return -1;
   const bool bf16 = words[kBf16];
   if (!operands_ok(a, bf16 ? 2 : 4, true)) return -2;
-  if (!grid_ok(a)) return -3;
+  if (!grid_ok(a, true)) return -3;
   void* out = (void*)words[kDtabOut];
   if ((a.dtab != nullptr) != (out != nullptr) || (out && !a.table)) return -4;
   a.ksplits = dtf_attention_bwd_splits(a.B, a.Sk, a.nh, a.nkv);

@@ -99,6 +99,30 @@ def test_attention_key_bias_in_64_bits(dt, Sq):
     _compare(q, k, v, do, key_bias=kb)
 
 
+# ------------------------------------------------------------------------------------------ large grids
+def test_few_queries_over_more_keys_than_the_other_kernels_grids_hold():
+    """One token of 32 heads over 2^25 keys of one head: 32 x 262145 tiles of 128 keys, which no kernel of this pass has as
+    its grid. A few keys far apart hold nearly all the weight. Bound: P and the result are rounded to bf16 (u); a score of 8
+    products 2 (8 + 8) u32 A; a lane adds at most 2^25 / (64 x 4 x 4) terms of P, a wave 2^25 / (64 x 4 x 32) products."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    nh, hd, Sk = 32, 8, (1 << 25) + 77
+    g = torch.Generator(DEV).manual_seed(4)
+    q = torch.randn(1, 1, nh, hd, device=DEV, generator=g).to(BF16)
+    k = (torch.randn(1, Sk, 1, hd, device=DEV, generator=g) * 0.1).to(BF16)
+    v = torch.randn(1, Sk, 1, hd, device=DEV, generator=g).to(BF16)
+    for i, at in enumerate((0, 5_000_000, (1 << 24) + 1, Sk - 78, Sk - 1)):
+        k[0, at, 0] = 60 * q[0, 0, 6 * i].float() / q[0, 0, 6 * i].float().norm() ** 2
+    out = attention(q, k, v)
+    t = q[0, 0].double() @ k[0, :, 0].double().t() / math.sqrt(hd)
+    A = q[0, 0].double().abs() @ k[0, :, 0].double().abs().t() / math.sqrt(hd)
+    p = torch.softmax(t, 1)
+    del t
+    want, u = p @ v[0, :, 0].double(), O.half_step(BF16)
+    terms = Sk // (64 * 4 * 4) + Sk // (64 * 4 * 32) + 512
+    tol = (p * (u + O.U32 * (2 * (hd + 8) * A + terms + 16))) @ v[0, :, 0].double().abs() + u * want.abs()
+    O.check("out", out[0, 0], want.cpu(), 1.01 * tol.cpu())
+
+
 # ------------------------------------------------------------------------------------------ the written bias
 @pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("cfg", [(3001, 2999, 20, 32, 128, True, None), (4099, 1501, 24, 16, 50, False, -900),
