@@ -47,6 +47,7 @@ struct Strided {                     // [B, S, heads, hd] with unit stride in hd
 };
 
 struct Args {
+  unsigned bytes;                    // sizeof(Args) where it was filled in: by_head_size refuses what another layout filled in
   Strided q, k, v, out, dout, dq, dk, dv;
   const float* key_bias;             // [B, Sk] or null
   const int* lens;                   // [B] or null
@@ -1685,6 +1686,7 @@ int run_bwd(const Args& a, hipStream_t stream) {
 }
 template <typename T, int MODE>
 int by_head_size(const Args& a, bool backward, hipStream_t s) {
+  if (a.bytes != sizeof(Args)) return -6;                // an object file of another state of this header
   if (a.hd <= 32) return backward ? run_bwd<T, 32, MODE>(a, s) : run_fwd<T, 32, MODE>(a, s);
   if (a.hd <= 64) return backward ? run_bwd<T, 64, MODE>(a, s) : run_fwd<T, 64, MODE>(a, s);
   if (a.hd <= 96) return backward ? run_bwd<T, 96, MODE>(a, s) : run_fwd<T, 96, MODE>(a, s);

@@ -18,6 +18,7 @@ enum Word {
 
 bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   if (n_words < kThr) return false;
+  a.bytes = sizeof(attn::Args);
   attn::Strided* t[8] = {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv};
   for (int i = 0; i < 8; ++i) {
     t[i]->p = (void*)w[kTensors + 4 * i];
@@ -58,11 +59,12 @@ bool unpack(const long long* w, int n_words, float scale, attn::Args& a) {
   if (!(scale > 0.f) || scale > 1e30f || a.hd % 8 || a.hd > 128 || a.nh % a.nkv) return false;
   if (a.table) {
     a.n_thr = a.half - a.exact - 1;
-    if (a.exact < 1 || a.buckets > 128 || a.max_dist <= a.exact || a.max_dist > 2048 || a.n_thr >= attn::kMaxThr ||
-        n_words < kThr + a.n_thr)
+    if (a.exact < 1 || a.buckets > 128 || a.max_dist <= a.exact || a.max_dist > 2048 || a.n_thr >= attn::kMaxThr || a.n_thr < 0)
       return false;
-    for (int i = 0; i < a.n_thr; ++i) a.thr[i] = (int)w[kThr + i];
   }
+  // no word missing and none too many: a caller with another order of words is refused, whatever it takes a word for
+  if (n_words != kThr + a.n_thr) return false;
+  for (int i = 0; i < a.n_thr; ++i) a.thr[i] = (int)w[kThr + i];
   return true;
 }
 

@@ -43,3 +43,24 @@ def test_attention_key_bias_in_64_bits():
     # a mean of 8 numbers: 8 roundings of 2^-24 of their magnitudes, and the softmax's few
     assert float((out[0] - v[0, alone].mean(0)).abs().max()) <= 32 * 2.0 ** -24 * float(v.abs().max())
     assert torch.equal(out[1], v[1, 2].expand(3, 2, 16))
+
+
+@pytest.mark.parametrize("table", [False, True])
+def test_a_call_with_other_words_is_refused(table):
+    """A word too few or too many (another order of them, that is) is an error code, before anything is launched. The right
+    number comes past that check, to the one of the operands, which are none here."""
+    import ctypes
+    import struct
+    from distributed_tensorflow_amd.ops.relative_bias import bucket_borders
+    words = [0] * 55
+    words[45:51] = (1, 1, 1, 1, 1, 8)                        # B, Sq, Sk, nh, nkv, hd
+    if table:
+        words[36:41] = (64, 0, 32, 128, 1)
+        words += bucket_borders(32, 128, True)
+    lib = _lib.kernels()
+    for name in ("dtf_attention_fwd", "dtf_attention_bwd"):
+        fn = getattr(lib, name)
+        for more in (-1, 1):
+            w = (words + [0])[: len(words) + more]
+            assert fn(struct.pack(f"{len(w)}q", *w), len(w), ctypes.c_float(1.0), None) == -1
+        assert fn(struct.pack(f"{len(words)}q", *words), len(words), ctypes.c_float(1.0), None) == -2
