@@ -99,6 +99,43 @@ def test_attention_key_bias_in_64_bits(dt, Sq):
     _compare(q, k, v, do, key_bias=kb)
 
 
+# ------------------------------------------------------------------------------------------ few queries
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Sk", [200, 1700], ids=["one_piece", "split"])
+@pytest.mark.parametrize("Sq,nh", [(1, 4), (5, 8), (16, 4)], ids=["2_rows", "20_rows", "32_rows"])
+@pytest.mark.parametrize("rel", [0, 16])
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+def test_few_queries_with_key_biases_and_garbage_behind_masks(dt, Sk, Sq, nh, rel, causal):
+    """-inf keys with NaN and infinities behind them, alone, with lengths and with a table; rows that no key is left for."""
+    B, nkv, hd = 5, 2, 64
+    q, k, v, do, table = _inputs(B, Sq, Sk, nh, nkv, hd, dt, rel, seed=8)
+    kb = torch.randn(B, Sk, generator=torch.Generator().manual_seed(2))
+    kb[0, ::3] = -math.inf
+    kb[1] = -math.inf
+    kb[2, 1:] = -math.inf
+    kb[3, :150] = -math.inf
+    for b, value in ((0, math.nan), (1, math.inf), (2, -math.inf), (3, math.nan)):
+        k[b, kb[b] == -math.inf], v[b, kb[b] == -math.inf] = value, value
+    n = torch.tensor([Sk, Sk - 9, Sk, Sk - 40, 0], dtype=torch.int32)
+    for b, m in enumerate(n.tolist()):
+        k[b, m:], v[b, m:], kb[b, m:] = math.nan, math.inf, math.nan
+    # (causal needs finite K and V where only it hides them: the queries are the last, or stand where every key that they do
+    # not see is masked anyway)
+    out, got = _compare(q, k, v, do, table, causal=causal, key_bias=kb, key_lengths=n, q_start=n - Sq if causal else None,
+                        rel_max_distance=60)
+    for b in (1, 4):
+        assert not out[b].any() and not any(g[b].any() for g in got[:3])
+
+
+@pytest.mark.parametrize("Sq,nh", [(1, 4), (5, 8), (16, 4), (33, 2)], ids=["2_rows", "20_rows", "32_rows", "66_rows"])
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cfg", [(32, 128, True), (128, 2048, False), (4, 3, True)], ids=str)
+def test_few_queries_with_a_table(dt, Sq, nh, cfg):
+    q, k, v, do, table = _inputs(2, Sq, 1100, nh, 2 if nh > 2 else 1, 96, dt, cfg[0])
+    _compare(q, k, v, do, table, causal=not cfg[2], rel_max_distance=cfg[1], rel_bidirectional=cfg[2],
+             q_start=torch.tensor([1100 - Sq, 500]))
+
+
 # ------------------------------------------------------------------------------------------ large grids
 def test_few_queries_over_more_keys_than_the_other_kernels_grids_hold():
     """One token of 32 heads over 2^25 keys of one head: 32 x 262145 tiles of 128 keys, which no kernel of this pass has as
@@ -121,6 +158,27 @@ def test_few_queries_over_more_keys_than_the_other_kernels_grids_hold():
     terms = Sk // (64 * 4 * 4) + Sk // (64 * 4 * 32) + 512
     tol = (p * (u + O.U32 * (2 * (hd + 8) * A + terms + 16))) @ v[0, :, 0].double().abs() + u * want.abs()
     O.check("out", out[0, 0], want.cpu(), 1.01 * tol.cpu())
+
+
+# ------------------------------------------------------------------------------------------ parts of the gradients
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("fused", [False, True], ids=["separate", "fused"])
+def test_attention_gradients_of_some_inputs(dt, fused):
+    """Any subset of q, k, v and the table may ask for its gradient: the same numbers as together."""
+    from distributed_tensorflow_amd.ops.attention import attention, self_attention
+    q, k, v, do, table = (t.to(DEV) for t in _inputs(2, 140, 140, 4, 2, 64, dt, 16))
+    ins = [torch.cat((q, k, v), 2), table] if fused else [q, k, v, table]
+
+    def grads(wanted):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(ins)]
+        out = self_attention(leaves[0], kv_heads=2, causal=True, rel_table=leaves[1]) if fused else \
+            attention(*leaves[:3], causal=True, rel_table=leaves[3])
+        return torch.autograd.grad(out, [leaves[i] for i in wanted], do)
+
+    every = grads(range(len(ins)))
+    for bits in range(1, 1 << len(ins)):
+        wanted = [i for i in range(len(ins)) if bits >> i & 1]
+        assert all(torch.equal(a, every[i]) for i, a in zip(wanted, grads(wanted))), wanted
 
 
 # ------------------------------------------------------------------------------------------ the written bias
