@@ -469,6 +469,16 @@ __device__ __forceinline__ int xcd_contiguous(int bid, int n) {
 // derived from it stays there unless told)
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Position of a batch element's first query, and how many keys any of its queries sees: what lies behind is never read, and
+// has zero gradients (the unfilled end of a cache may hold anything)
+__device__ __forceinline__ int first_position(const Args& a, int b) {
+  return uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
+}
+__device__ __forceinline__ int used_keys(const Args& a, int b, int start) {
+  const int n = a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk;
+  return uni(a.causal ? min(n, max(start + a.Sq, 0)) : n);
+}
+
 // Workgroup -> (sequence, tile): `pairs` sequences (a batch element's head) of n tiles each. Tiles of one sequence stay on
 // one XCD. Causal tiles are of unequal work, rank 0 the longest: rank by rank then, the longest of all sequences first, so
 // that what comes last is short; when all workgroups are resident at once (at most two a CU) the second half of the ranks
@@ -506,8 +516,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
   const int b = uni(bh / a.nh), h = bh - b * a.nh, qt = a.causal ? nqt - 1 - rank : rank;
   const int kvh = uni(h / (a.nh / a.nkv));
   const int q0 = qt * kRows + wid * 32;
-  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
-  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
+  const int start = first_position(a, b), klen = used_keys(a, b, start);
   const int pos0 = start + q0;
   const float c = a.score_scale * kLog2e;
   const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
@@ -773,8 +782,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
   float* tab = ml + 4 * 2 * QB * 16;
   const int group = uni(a.nh / a.nkv), rows = a.Sq * group;
   const int bk = uni(blockIdx.x / a.splits), split = blockIdx.x - bk * a.splits, b = uni(bk / a.nkv), kvh = bk - b * a.nkv;
-  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
-  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
+  const int start = first_position(a, b), klen = used_keys(a, b, start);
   const float c = a.score_scale * kLog2e;
   const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
@@ -1082,8 +1090,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
   const int b = uni(bh / a.nh), h = bh - b * a.nh, qt = a.causal ? nqt - 1 - rank : rank;
   const int kvh = uni(h / (a.nh / a.nkv));
   const int q0 = qt * kRows + wid * 32;
-  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
-  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
+  const int start = first_position(a, b), klen = used_keys(a, b, start);
   const int pos0 = start + q0;
   const float c = a.score_scale * kLog2e;
   const T* qp = (const T*)a.q.p + b * a.q.sb + h * a.q.sh;
@@ -1355,8 +1362,7 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 32 ? 4 : D <=
   place(a.B * a.nkv * a.ksplits, nkt, a.causal, pair, rank);
   const int bk = uni(pair / a.ksplits), b = uni(bk / a.nkv), kvh = bk - b * a.nkv, split = pair - bk * a.ksplits;
   const int heads = uni(group / a.ksplits), kb0 = rank * kRows, k0 = kb0 + wid * 32;
-  const int klen = uni(a.lens ? min(max(a.lens[b], 0), a.Sk) : a.Sk);
-  const int start = uni(a.q_start ? min(max(a.q_start[b], -kMaxStart), kMaxStart) : a.q_start0);
+  const int start = first_position(a, b), klen = used_keys(a, b, start);
   const float c = a.score_scale * kLog2e;
   const T* kp = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
   const T* vp = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;

@@ -318,9 +318,11 @@ def _composed(q, k, v, table, key_bias, lens, starts, nkv, opts):
         ok &= torch.arange(Sk) < lens[:, None]
     if key_bias is not None:
         ok &= key_bias != -math.inf
+    first = torch.full((B,), start0) if starts is None else starts.long()
+    if causal:
+        ok &= torch.arange(Sk) < (first + Sq)[:, None]         # (nothing behind the last query is read)
     k, v = (t.float().masked_fill(~ok[:, :, None, None], 0.0).transpose(1, 2).repeat_interleave(nh // nkv, 1) for t in (k, v))
     t = q.float().transpose(1, 2) @ k.transpose(2, 3) * scale
-    first = torch.full((B,), start0) if starts is None else starts.long()
     dist = torch.arange(Sk) - (torch.arange(Sq)[:, None] + first[:, None, None])               # [B, Sq, Sk]
     if table is not None:
         bucket = _rel.relative_bucket(dist, table.shape[0], max_distance, bidirectional)
@@ -405,7 +407,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_bias: torch
     ``rel_table[buckets, nh]`` adds the learned bias of ``ops/relative_bias.py`` for the distance to that position
     (``rel_bidirectional`` defaults to ``not causal``). A query that no key is left for gets zeros, and zero gradients.
 
-    K and V of keys that only ``causal`` hides have to be finite. On a GPU forward-mode derivatives and traces are refused."""
+    With ``causal`` what lies behind the last query's position is never used either (the unfilled end of a cache); K and V
+    of the keys up to it have to be finite, though earlier queries do not see them all. On a GPU forward-mode derivatives
+    and traces are refused."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError(f"q[B, Sq, nh, hd] and k, v[B, Sk, nkv, hd] do not fit: {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")

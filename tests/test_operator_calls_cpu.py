@@ -64,3 +64,21 @@ def test_a_call_with_other_words_is_refused(table):
             w = (words + [0])[: len(words) + more]
             assert fn(struct.pack(f"{len(w)}q", *w), len(w), ctypes.c_float(1.0), None) == -1
         assert fn(struct.pack(f"{len(words)}q", *words), len(words), ctypes.c_float(1.0), None) == -2
+
+
+@pytest.mark.parametrize("Sq,Sk", [(1, 9), (4, 11)])
+def test_attention_over_the_filled_part_of_a_cache(Sq, Sk):
+    """NaN and infinities behind the last query's position, without key_lengths: causal alone keeps them out, of the result
+    and of the gradients."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    filled = torch.tensor([Sk, Sq, Sk - 3], dtype=torch.int32)
+    q, k, v = (torch.randn(3, n, 2, 16, generator=torch.Generator().manual_seed(n)) for n in (Sq, Sk, Sk))
+    runs = []
+    for fill in (0.0, torch.nan):
+        kk, vv = k.clone(), v.clone()
+        for b, n in enumerate(filled.tolist()):
+            kk[b, n:], vv[b, n:] = fill, fill
+        leaves = [t.clone().requires_grad_() for t in (q, kk, vv)]
+        out = attention(*leaves, causal=True, q_start=filled - Sq)
+        runs.append([out, *torch.autograd.grad(out.sum(), leaves)])
+    assert all(torch.equal(a, b) for a, b in zip(*runs)) and torch.isfinite(runs[0][0]).all()

@@ -10,7 +10,7 @@ from torch.autograd import forward_ad as fwAD
 
 sys.path.insert(0, os.path.dirname(__file__))
 import operator_oracles as O  # noqa: E402
-from test_operators_gpu import BF16, DEV, FP32, _compare, _compare_logp, _inputs, _logits  # noqa: E402
+from test_operators_gpu import BF16, DEV, FP32, _compare, _compare_logp, _dev, _inputs, _logits  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -134,6 +134,36 @@ def test_few_queries_with_a_table(dt, Sq, nh, cfg):
     q, k, v, do, table = _inputs(2, Sq, 1100, nh, 2 if nh > 2 else 1, 96, dt, cfg[0])
     _compare(q, k, v, do, table, causal=not cfg[2], rel_max_distance=cfg[1], rel_bidirectional=cfg[2],
              q_start=torch.tensor([1100 - Sq, 500]))
+
+
+# ------------------------------------------------------------------------------------------ unfilled caches
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Sq,Sk", [(1, 90), (1, 2000), (7, 700), (150, 300)], ids=str)
+@pytest.mark.parametrize("extra", ["", "table", "key_bias", "lengths"])
+def test_attention_over_the_filled_part_of_a_cache(dt, Sq, Sk, extra):
+    """NaN and infinities behind the last query's position, without key_lengths: causal alone keeps them out, of the result
+    and of the gradients."""
+    B, nh, nkv, hd = 4, 4, 2, 64
+    q, k, v, do, table = _inputs(B, Sq, Sk, nh, nkv, hd, dt, 16 if extra == "table" else 0, seed=11)
+    filled = torch.tensor([Sk, Sq, Sk // 2 + 5 if Sq < 100 else 260, Sk - 1], dtype=torch.int32)
+    kw = {}
+    if extra == "key_bias":
+        kw["key_bias"] = torch.randn(B, Sk, generator=torch.Generator().manual_seed(3))
+    if extra == "lengths":
+        kw["key_lengths"] = torch.tensor([Sk, Sk, Sk // 2, 1], dtype=torch.int32)
+    clean = [t.clone() for t in (k, v)]
+    for b, n in enumerate(filled.tolist()):
+        k[b, n:], v[b, n:] = math.nan, math.inf
+        for t in clean:
+            t[b, n:] = 0
+    from distributed_tensorflow_amd.ops.attention import attention
+    kw.update(causal=True, q_start=filled - Sq)
+    val, tol = O.attention(q, *clean, do, rel_table=table, **kw)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)] + ([] if table is None else [table.to(DEV).requires_grad_()])
+    out = attention(*leaves[:3], rel_table=None if table is None else leaves[3], **{n: _dev(x) for n, x in kw.items()})
+    O.check("out", out, val["out"], tol["out"])
+    for n, g in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, do.to(DEV))):
+        O.check(n, g, val[n], tol[n])
 
 
 # ------------------------------------------------------------------------------------------ large grids
