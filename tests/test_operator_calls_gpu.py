@@ -274,3 +274,63 @@ def test_token_log_probs_of_subnormal_logits(dt):
     x[2, :100] = -tiny / 2
     gs = (torch.randn(6, generator=g), torch.randn(6, generator=g), torch.randn(6, 9, generator=g))
     _compare_logp(x, tok, 9, gs)
+
+
+# ------------------------------------------------------------------------------------------ offsets beyond 32 bits
+def test_token_log_probs_beyond_32_bits():
+    """70001 x 32000 logits: the last rows are those of a call on them alone."""
+    from distributed_tensorflow_amd.ops.softmax_ce import token_log_probs
+    N, V, n = 70001, 32000, 777
+    x = torch.randn(N, V, dtype=BF16, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    tok = torch.randint(0, V, (N,), device=DEV)
+
+    def run(x, tok):
+        x = x.detach().requires_grad_()
+        r = token_log_probs(x, tok, 3)
+        d, = torch.autograd.grad((r.logp.sum(), r.entropy.sum(), r.top_logp.sum()), x)
+        return [*r, d]
+
+    assert all(torch.equal(a[-n:], b) for a, b in zip(run(x, tok), run(x[-n:].clone(), tok[-n:])))
+
+
+def test_relative_bias_beyond_32_bits():
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    q_len, k_len, heads, buckets = 12001, 11987, 16, 32
+    table = torch.randn(buckets, heads, dtype=BF16, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).requires_grad_()
+    out = relative_bias(table, q_len, k_len)
+    low = -(q_len - 1) - (k_len - q_len)
+    of = O.buckets_between(low, q_len - 1, buckets, 128, True).to(DEV)
+    assert torch.equal(out[-1], table[:, -1][of].unfold(0, k_len, 1).flip(0))
+    # the gradient where only the last head's last rows count: those rows' elements, whole numbers, added exactly
+    g = torch.zeros_like(out)
+    g[-1, -5:] = 1
+    got, = torch.autograd.grad(out, table, g)
+    want = torch.zeros(buckets, heads, device=DEV)
+    for i in range(q_len - 5, q_len):
+        want[:, -1] += torch.bincount(of[q_len - 1 - i:q_len - 1 - i + k_len], minlength=buckets)
+    assert torch.equal(got, want.to(BF16))
+
+
+@pytest.mark.parametrize("fused", [False, True], ids=["separate", "fused"])
+def test_attention_beyond_32_bits(fused):
+    """41 x 8192 x 64 heads of 128, few keys: the last sequences are those of a call on them alone (the same kernel variants
+    in the same order of sums)."""
+    from distributed_tensorflow_amd.ops.attention import attention, self_attention
+    B, S, nh, hd, n = (41, 8192, 64, 128, 6) if not fused else (700, 200, 64, 128, 90)
+    g = torch.Generator(DEV).manual_seed(3)
+    if fused:
+        ins = [torch.randn(B, S, 3 * nh, hd, dtype=BF16, device=DEV, generator=g)]
+    else:
+        ins = [torch.randn(B, s, nh, hd, dtype=BF16, device=DEV, generator=g) for s in (S, 100, 100)]
+    do = torch.randn(B, S, nh, hd, dtype=BF16, device=DEV, generator=g)
+    lens = torch.randint(1, 100, (B,), device=DEV, dtype=torch.int32)
+    assert ins[0].numel() > 1 << 31
+
+    def run(ins, do, lens):
+        ins = [t.detach().requires_grad_() for t in ins]
+        out = self_attention(*ins, kv_heads=nh, key_lengths=lens) if fused else attention(*ins, key_lengths=lens)
+        return [out, *torch.autograd.grad(out, ins, do)]
+
+    whole = run(ins, do, lens)
+    part = run([t[-n:].clone() for t in ins], do[-n:].clone(), lens[-n:].clone())
+    assert all(torch.equal(a[-n:], b) for a, b in zip(whole, part))
