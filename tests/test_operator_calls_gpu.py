@@ -10,6 +10,7 @@ from torch.autograd import forward_ad as fwAD
 
 sys.path.insert(0, os.path.dirname(__file__))
 import operator_oracles as O  # noqa: E402
+from distributed_tensorflow_amd.engine.graph import collected  # noqa: E402
 from test_operators_gpu import BF16, DEV, FP32, _compare, _compare_logp, _dev, _inputs, _logits  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -164,6 +165,75 @@ def test_attention_over_the_filled_part_of_a_cache(dt, Sq, Sk, extra):
     O.check("out", out, val["out"], tol["out"])
     for n, g in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, do.to(DEV))):
         O.check(n, g, val[n], tol[n])
+
+
+# ------------------------------------------------------------------------------------------ distances masked by the table
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("mask", [-math.inf, torch.finfo(BF16).min], ids=["inf", "lowest"])
+@pytest.mark.parametrize("Sq,Sk", [(200, 200), (2, 900)], ids=["rows", "few"])
+@pytest.mark.parametrize("bias", [False, True], ids=["", "key_bias"])
+def test_attention_with_distances_that_the_table_masks(dt, mask, Sq, Sk, bias):
+    """-inf, or the type's lowest value, in some buckets, the far ones among them: the keys there take no part. (The oracle is
+    given -1e31, which leaves them none either: every row has other keys.)"""
+    q, k, v, do, table = _inputs(2, Sq, Sk, 4, 2, 64, dt, 16, seed=12)
+    table[7], table[15], table[3, 1], table[11] = mask, mask, mask, mask
+    low = table.clone()
+    low[table.float() < -1e30] = -1e31
+    kw = dict(rel_max_distance=30, rel_bidirectional=True)
+    if bias:
+        kw["key_bias"] = torch.randn(2, Sk, generator=torch.Generator().manual_seed(4))
+        kw["key_bias"][0, ::5] = -math.inf
+    from distributed_tensorflow_amd.ops.attention import attention
+    val, tol = O.attention(q, k, v, do, rel_table=low, **kw)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, table)]
+    out = attention(*leaves[:3], rel_table=leaves[3], **{n: _dev(x) for n, x in kw.items()})
+    O.check("out", out, val["out"], tol["out"])
+    for n, g in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, do.to(DEV))):
+        O.check(n, g, val[n], tol[n])
+    if mask == -math.inf:                                    # a head whose every distance is masked
+        with torch.no_grad():
+            leaves[3][:, 2] = mask
+        out = attention(*leaves[:3], rel_table=leaves[3], **{n: _dev(x) for n, x in kw.items()})
+        gq, gk, gv, gt = torch.autograd.grad(out, leaves, do.to(DEV))
+        assert not out[:, :, 2].any() and not gq[:, :, 2].any() and not gt[:, 2].any()
+        assert all(torch.isfinite(t).all() for t in (out, gq, gk, gv, gt))
+
+
+# ------------------------------------------------------------------------------------------ captured decoding
+@pytest.mark.parametrize("ints", [torch.int32, torch.int64], ids=["int32", "int64"])
+@pytest.mark.parametrize("table", [False, True], ids=["", "table"])
+def test_new_tokens_over_a_growing_cache_in_a_graph(ints, table):
+    """One captured call, replayed while the caches fill: lengths and starts are read anew from the caller's tensors."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    B, nh, nkv, hd, Sk = 3, 8, 2, 64, 1500
+    g = torch.Generator(DEV).manual_seed(5)
+    k, v = (torch.full((B, Sk, nkv, hd), math.nan, dtype=BF16, device=DEV) for _ in range(2))
+    q = torch.randn(B, 1, nh, hd, dtype=BF16, device=DEV, generator=g)
+    t = torch.randn(16, nh, dtype=BF16, device=DEV, generator=g) if table else None
+    n, at = (torch.zeros(B, dtype=ints, device=DEV) for _ in range(2))
+
+    def call():
+        return attention(q, k, v, causal=True, key_lengths=n, q_start=at, rel_table=t)
+
+    def fill(step):
+        for b, m in enumerate((1 + step, 700 * step, 1500 - step)):
+            k[b, :m] = torch.randn(m, nkv, hd, dtype=BF16, device=DEV, generator=g)
+            v[b, :m] = torch.randn(m, nkv, hd, dtype=BF16, device=DEV, generator=g)
+            n[b], at[b] = m, m - 1
+
+    fill(0)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with collected(), torch.cuda.graph(graph):
+        out = call()
+    for step in range(3):
+        fill(step)
+        q.mul_(-1.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call()) and torch.isfinite(out).all()
+        assert bool(out[1].any()) == (step > 0)              # (an empty cache gives zeros)
 
 
 # ------------------------------------------------------------------------------------------ large grids
