@@ -14,10 +14,11 @@
 // for either type; the order of the 32 elements is free as long as both operands agree on it).
 //
 // Scores are kept as step t for a factor step = unit / scale (unit 1: q . k as it is): the biases are multiplied by it where
-// they are staged and enter as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score.
-// Beside a key bias unit is the power of two below a scale under 1, and the operand that stays in registers carries it: step
-// is then at most 1, so any finite bias stays finite, and equal ones equal (1 / scale itself would carry a bias beyond 4.3e37
-// past the type's range at heads of 64). A power of two rounds nothing.
+// they are staged and enter as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score
+// (but in few_kernel, which finds the bucket of each score). Beside a key bias unit is the power of two below a scale under 1,
+// and the operand that stays in registers carries it: step is then at most 1, so any finite bias stays finite, and equal ones
+// equal (1 / scale itself would carry a bias beyond 4.3e37 past the type's range at heads of 64). A power of two rounds
+// nothing.
 //
 // Measured (bf16, us and the rate of the products): 64 x 512 tokens x 12 heads of 64, with a table: forward 111 (P in two
 // parts, see PARTS), dQ and dTable 174, dK / dV 157; without one 85, 111, 120 (605, 697, 862 TFLOP/s of what each has to do);
@@ -434,7 +435,7 @@ __device__ __forceinline__ void fill_band(const Args& a, int h, float* band, int
 }
 // What a kernel instance knows of the biases: none, the relative one alone, or a key bias with or without it.
 enum Mode { kPlain = 0, kRel = 1, kKeys = 2 };
-// Whether a forward pass may be asked for a table's gradient: then P enters O in two parts (see fwd_kernel).
+// Whether P may enter O in two parts (see fwd_kernel): it does where there is a table and any gradient is asked for.
 template <typename T, int MODE>
 constexpr bool two_parts() { return sizeof(T) == 2 && MODE != kPlain; }
 
@@ -482,7 +483,10 @@ __device__ __forceinline__ int used_keys(const Args& a, int b, int start) {
 // Workgroup -> (sequence, tile): `pairs` sequences (a batch element's head) of n tiles each. Tiles of one sequence stay on
 // one XCD. Causal tiles are of unequal work, rank 0 the longest: rank by rank then, the longest of all sequences first, so
 // that what comes last is short; when all workgroups are resident at once (at most two a CU) the second half of the ranks
-// goes the other way round, so that a long and a short one share a CU.
+// goes the other way round, so that a long and a short one share a CU. That deals sequences to the XCDs by eights: other
+// numbers of them are dealt in order, without regard to the work (causal 8192 tokens, heads of 64, forward / dQ / dK, dV:
+// 1 head 93 / 87 / 113 us, 4 heads 101 / 97 / 126, 8 heads 110 / 140 / 178, 12 heads 186 / 206 / 263, 16 heads 190 / 200 /
+// 255).
 __device__ __forceinline__ void place(int pairs, int n, bool causal, int& pair, int& rank) {
   const int bid = blockIdx.x;
   if (causal && !(pairs & 7)) {
@@ -500,7 +504,8 @@ __device__ __forceinline__ void place(int pairs, int n, bool causal, int& pair, 
 // PARTS 2: P enters O as two bf16 numbers, its rounding and what that left. D = rowsum(dO * O) takes over the roundings of the
 // P in O, each row's one error in all of its dT, and the sums over many rows in a table's gradient show it (relative error
 // against 64 bits 0.0015 to 0.0033 with one part, 0.0012 to 0.0018 with two, most of that dTable's own rounding; dQ and
-// dK, rounded more coarsely by themselves, keep theirs). 64 x 512 x 12 heads of 64: 91 us with one part, 111 with two.
+// dK, rounded more coarsely by themselves, keep theirs). 64 x 512 x 12 heads of 64: 91 us with one part, 111 with two. The pass
+// is told that gradients are asked for, not which: with a table that takes none it is two as well.
 template <typename T, int D, int MODE, int GROUPS, int PARTS>
 __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) : (D <= 64 ? 2 : GROUPS))) void fwd_kernel(Args a) {
   constexpr int KT = key_tile<T>(), JB = KT / 16, DB = D / 16, DS = D / 32, IMG = Tile<T, D, KT>::IMG;
@@ -750,6 +755,9 @@ __global__ __launch_bounds__(256 * GROUPS, (sizeof(T) == 2 ? (D <= 64 ? 4 : 2) :
 // LDS image of the wave's own, and no barrier stands in the loop. All query heads of a key head ride in one tile of rows,
 // so the cache is read once, not once a query head. The waves' (maximum, sum, O) join in the LDS, the workgroups' in a
 // second kernel.
+// 8 x 1 on 4001 keys, 16 heads on 4 of 128, the two kernels, us: bf16 13 + 4 (floor 9: two tiles a wave, so that the start, the
+// join and the second launch dominate), fp32 28 + 5; with key biases 20 and 45. The bucket of each score is found border by
+// border: with a one-sided table of 32 buckets 23 and 38, of 128 49 and 64.
 constexpr int kFewRows = 32, kFewKeys = 32;
 
 // O and the row's statistics of row r of a key head's rows
@@ -1611,6 +1619,9 @@ inline int launch(K kernel, long long blocks, int threads, int lds, const Args& 
 // Key splits of the few-queries path: two workgroups a CU, and at least two key tiles for each of a workgroup's waves
 // (fewer and the joining costs more than the splitting gains; 8 sequences x 4001 keys, 16 heads on 4 of 128: 12 + 4 us
 // against 100 unsplit). 1: no second kernel.
+// Which calls: up to 32 rows (queries x heads of a group), as many as few_kernel's tile holds. The other kernels do not split
+// the keys, so over a long cache they leave most CUs without work; both sides of the border, us, heads of 128, 16 on 4, causal:
+// 1 x 8 on 20000 (32 rows) 13 + 6, 1 x 9 279, 1 x 128 287; 8 x 8 on 4001 18 + 4, 8 x 9 62, 8 x 128 69.
 inline bool few_queries(int Sq, int nh, int nkv) { return (long long)Sq * (nh / nkv) <= kFewRows; }
 inline int few_splits(int B, int Sk, int nkv) {
   const long long groups = (long long)B * nkv, most = (Sk + 8 * kFewKeys - 1) / (8 * kFewKeys);

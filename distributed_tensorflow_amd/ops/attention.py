@@ -405,7 +405,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_bias: torch
     (default: the queries are the last ``Sq`` of ``Sk`` positions; a tensor ``[B]`` gives each sequence its own, as for
     new tokens over caches filled to different lengths). ``causal``: keys after the query's position take no part.
     ``rel_table[buckets, nh]`` adds the learned bias of ``ops/relative_bias.py`` for the distance to that position
-    (``rel_bidirectional`` defaults to ``not causal``). A query that no key is left for gets zeros, and zero gradients.
+    (``rel_bidirectional`` defaults to ``not causal``); ``-inf`` in it masks a bucket's distances, other values count up to
+    1.1e7 either way. A query that no key is left for gets zeros, and zero gradients.
 
     With ``causal`` what lies behind the last query's position is never used either (the unfilled end of a cache); K and V
     of the keys up to it have to be finite, though earlier queries do not see them all. On a GPU forward-mode derivatives
