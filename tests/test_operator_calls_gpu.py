@@ -346,6 +346,26 @@ def test_token_log_probs_of_subnormal_logits(dt):
     _compare_logp(x, tok, 9, gs)
 
 
+# ------------------------------------------------------------------------------------------ logits far from zero
+@pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N,V", [(9, 353), (9, 5003), (9, 30522), (600, 6001)])
+def test_token_log_probs_of_logits_far_from_zero(dt, N, V):
+    """What all logits of a row have in common leaves no trace: rows of nothing but the type's lowest value or its largest, rows
+    far from zero either way, and rows masked to few by the lowest value."""
+    x, tok, g = _logits(N, V, dt)
+    x[0] = torch.finfo(dt).min
+    x[1] = torch.finfo(dt).max
+    for i, off in ((2, 3e4), (3, -3e4), (4, 1e6), (5, -1e20)):
+        x[i] = (x[i].float() + off).to(dt)
+    x[6] = torch.finfo(dt).min
+    x[6, V // 2:V // 2 + 3] = x[2, :3]
+    x[7] = torch.finfo(dt).min
+    x[7, 5::7] = 1.0
+    tok[6] = V // 2 + 1
+    gs = (torch.randn(N, generator=g), torch.randn(N, generator=g), torch.randn(N, 9, generator=g))
+    _compare_logp(x, tok, 9, gs)
+
+
 # ------------------------------------------------------------------------------------------ offsets beyond 32 bits
 def test_token_log_probs_beyond_32_bits():
     """70001 x 32000 logits: the last rows are those of a call on them alone."""
