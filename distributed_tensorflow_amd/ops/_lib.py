@@ -13,6 +13,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -135,6 +136,19 @@ def differentiated(*tensors: torch.Tensor | None) -> bool:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+_packs: dict = {}
+
+
+def pack_words(words) -> bytes:
+    """64-bit words as a C entry reads them. (A packer a length: struct.pack itself is one that torch.compile replaces, by a
+    function that never ends.)"""
+    n = len(words)
+    pack = _packs.get(n)
+    if pack is None:
+        pack = _packs[n] = struct.Struct(f"{n}q").pack
+    return pack(*words)
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -21,7 +21,6 @@ from __future__ import annotations
 import ctypes
 import math
 import os
-import struct
 
 import torch
 
@@ -164,7 +163,7 @@ def _call(name: str, words, scale: float, like: torch.Tensor) -> None:
         _entry[name] = fn
     n = len(words)
     with _lib.on_device(like):
-        rc = fn(struct.pack(f"{n}q", *words), n, scale, _lib.stream_ptr(like.device))
+        rc = fn(_lib.pack_words(words), n, scale, _lib.stream_ptr(like.device))
     if rc:
         _lib.check(rc, name)
 

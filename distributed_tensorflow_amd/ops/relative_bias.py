@@ -17,7 +17,6 @@ exact^(half - exact)``), so a distance that lies on a border is not decided by r
 """
 from __future__ import annotations
 
-import struct
 from functools import lru_cache
 
 import torch
@@ -71,7 +70,7 @@ def relative_bucket(distance: torch.Tensor, buckets: int, max_distance: int = 12
 def _words(q_len: int, k_len: int, heads: int, q_start: int, buckets: int, max_distance: int, bidirectional: bool):
     w = (q_len, k_len, heads, q_start, buckets, max_distance, int(bidirectional),
          *bucket_borders(buckets, max_distance, bidirectional))          # (the sizes of a call as its C entry reads them)
-    return struct.pack(f"{len(w)}q", *w), len(w)
+    return _lib.pack_words(w), len(w)
 
 
 def _forward(table, q_len, k_len, q_start, max_distance, bidirectional):

@@ -56,6 +56,29 @@ def test_a_trace_is_refused_and_not_left_without_the_kernels():
             torch.jit.trace(call, (ins[0].detach().clone().requires_grad_(), *ins[1:]))
 
 
+# ------------------------------------------------------------------------------------------ inside a compiled function
+def test_calls_inside_a_compiled_function():
+    """torch.compile breaks its graph around the kernels: the same results and gradients as without it."""
+    from distributed_tensorflow_amd.ops.attention import attention
+    from distributed_tensorflow_amd.ops.relative_bias import relative_bias
+    from distributed_tensorflow_amd.ops.softmax_ce import token_log_probs
+    q, k, v, _, table = (t.to(DEV) for t in _inputs(2, 40, 50, 2, 1, 16, FP32, 8))
+    tok = torch.arange(16, device=DEV)
+    for call in (lambda q, k, v, t: attention(q * 1, k, v, causal=True, rel_table=t) + 1,
+                 lambda q, k, v, t: attention(q[:, :1] * 1, k, v, rel_table=t) + 1,
+                 lambda q, k, v, t: relative_bias(t * 2, 9, 12) + 1,
+                 lambda q, k, v, t: token_log_probs(q.reshape(16, 160) * 1, tok, 2).logp + 1):
+        torch._dynamo.reset()
+        fast, runs = torch.compile(call, backend="eager"), []
+        for f in (call, fast):
+            leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+            out = f(*leaves)
+            grads = torch.autograd.grad(out.sum(), leaves, allow_unused=True)
+            with torch.no_grad():
+                runs.append([out, f(*leaves), *(g for g in grads if g is not None)])
+        assert len(runs[0]) == len(runs[1]) and all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 # ------------------------------------------------------------------------------------------ key biases at the ends of their type
 @pytest.mark.parametrize("dt", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("Sq,Sk", [(70, 90), (3, 700)], ids=["rows", "few"])
