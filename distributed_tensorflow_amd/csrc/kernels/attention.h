@@ -13,8 +13,8 @@
 // v_mfma_f32_16x16x4_f32, eight of which cover the same 32 contraction elements (Frag below holds 8 elements of a lane
 // for either type; the order of the 32 elements is free as long as both operands agree on it).
 //
-// Scores are kept as step t for a factor step = unit / scale (unit 1: q . k as it is): the biases are multiplied by it where
-// they are staged and enter as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score
+// Scores are kept as step * t, step = unit / scale (unit 1: q . k as it is): the biases are multiplied by step where they are
+// staged and enter as the INITIAL VALUE of the score accumulators, so a bias costs no vector instruction per score
 // (but in few_kernel, which finds the bucket of each score). Beside a key bias unit is the power of two below a scale under 1,
 // and the operand that stays in registers carries it: step is then at most 1, so any finite bias stays finite, and equal ones
 // equal (1 / scale itself would carry a bias beyond 4.3e37 past the type's range at heads of 64). A power of two rounds
